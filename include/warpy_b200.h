@@ -39,6 +39,7 @@ extern "C" {
 /* dtype codes */
 #define WK_BF16 0
 #define WK_F32 1
+#define WK_F16 2
 
 /* Replaces warpy_kernels/arch.py:69-94 (supports): 1 if `feature` ("gemm",
  * "gemm_fp8", "gemm_mx", "gemm_mx_out", "attn_fwd_fp8", "attn_bwd_fp8", ...) has a
@@ -310,6 +311,63 @@ int wk_attn_bwd_fp8(const wk_attn_bwd_args* args, void* stream);
  * launches for 16-bit inputs (warpy_kernels/attn/bwd_api.py:381-398, bwd_sm120.py:436-464). */
 int64_t wk_attn_bwd_bf16_workspace_bytes(int B, int Hq, int Nq);
 int wk_attn_bwd_bf16(const wk_attn_bwd_args* args, void* stream);
+
+/* Position rotation of queries and keys, with or without the RMS norm of every head before it.  No counterpart in the
+ * reference, whose callers hand finished q and k to attn_fwd; these are the passes before that call.
+ *   u = x                                      (q_weight NULL)
+ *   u = x . (mean(x^2) + eps)^-1/2 . weight    (over the d elements of a head)
+ *   q_out = R(theta) u, or e4m3(R(theta) u / q_descale) when q_descale is given; the same for k
+ * R turns the pairs (j, j + rot / 2) of the first rot elements, or (2 j, 2 j + 1) when interleaved, by
+ * theta_j = positions[axis(j)][b][n] * inv_freq[j] (back when inverse); elements from rot on are not turned.
+ *   q [B,Hq,N,d], k [B,Hk,N,d] (Hk == 0: no keys)  dtype WK_BF16, WK_F16 or WK_F32; q_out, k_out of the same dtype, or
+ *       e4m3 bytes.  *_strides = element strides of dims (B, H, N), the last dimension contiguous; base and strides
+ *       multiples of 16 bytes (8 for e4m3 outputs).  An output may be its own input (same base and strides) but must
+ *       not overlap anything else
+ *   q_weight, k_weight [d]  contiguous, dtype w_dtype
+ *   q_descale, k_descale    fp32 [B,Hkv] contiguous, as the FP8 attention takes them (value = code . descale);
+ *       Hq % Hkv == 0, Hk == Hkv (or 0)
+ *   positions [axes][B][N]  int32 or int64, element strides position_strides
+ *   axis_map                axis of pair j in bits 2 (j % 32) of word j / 32
+ *   inv_freq [rot / 2]      fp32 or fp64, contiguous
+ * d a multiple of 16 from 32 to 256, rot a multiple of 16 up to d. */
+typedef struct {
+  const void* q;
+  const void* k;
+  void* q_out; /* backward: gradients of q and k */
+  void* k_out;
+  const void* q_weight;
+  const void* k_weight;
+  const float* q_descale;
+  const float* k_descale;
+  const void* positions;
+  const void* inv_freq;
+  const void* dq_out; /* backward: gradients of the outputs, dtype of q */
+  const void* dk_out;
+  void* dq_weight; /* backward: [d], dtype w_dtype */
+  void* dk_weight;
+  void* workspace; /* backward: wk_qk_norm_rope_bwd_workspace_bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t q_strides[3];
+  int64_t k_strides[3];
+  int64_t q_out_strides[3];
+  int64_t k_out_strides[3];
+  int64_t dq_out_strides[3];
+  int64_t dk_out_strides[3];
+  int64_t position_strides[3];
+  uint64_t axis_map[4];
+  int32_t B, N, Hq, Hk, Hkv, d, rot;
+  int32_t dtype, w_dtype;
+  int32_t position_int64, inv_freq_f64;
+  int32_t interleaved, inverse;
+  float eps;
+} wk_rope_args;
+
+int wk_rope(const wk_rope_args* args, void* stream);
+
+/* Gradients of the call above with weights: q_out, k_out receive the gradients of q and k; dq_weight, dk_weight those of
+ * the weights, summed in fp32 in a fixed order.  q_descale, k_descale NULL; heads = Hq + Hk. */
+int64_t wk_qk_norm_rope_bwd_workspace_bytes(int B, int N, int heads, int d);
+int wk_qk_norm_rope_bwd(const wk_rope_args* args, void* stream);
 
 #ifdef __cplusplus
 }

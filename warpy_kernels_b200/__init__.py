@@ -3,6 +3,7 @@
 from .arch import device_arch, supports
 from .interface import attn_bwd, attn_fwd, autotune_gemm, gemm, make_gemm
 from .quant import quantize_mx
+from .rotary import qk_norm_rope, qk_norm_rope_bwd, rope
 
 __all__ = [
     "attn_bwd",
@@ -11,6 +12,9 @@ __all__ = [
     "device_arch",
     "gemm",
     "make_gemm",
+    "qk_norm_rope",
+    "qk_norm_rope_bwd",
     "quantize_mx",
+    "rope",
     "supports",
 ]

@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("WARPY_KERNELS_B200_LIB") or os.path.join(_HERE, "libw
 
 _i32, _i64, _ptr, _str = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_char_p
 
-WK_BF16, WK_F32 = 0, 1
+WK_BF16, WK_F32, WK_F16 = 0, 1, 2
 
 # name -> (restype, argtypes); must list every function the header declares
 SIGNATURES = {
@@ -42,6 +42,9 @@ SIGNATURES = {
     "wk_gemm_mxfp8_noalloc": (_i32, [_ptr, _ptr]),
     "wk_gemm_mxfp8_noalloc_max_bytes": (_i64, []),
     "wk_gemm_mxfp8_noalloc_status": (_i32, []),
+    "wk_rope": (_i32, [_ptr, _ptr]),
+    "wk_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i32] * 4),
+    "wk_qk_norm_rope_bwd": (_i32, [_ptr, _ptr]),
 }
 
 _lib = None

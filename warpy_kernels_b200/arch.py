@@ -14,10 +14,11 @@ ARCH = 100
 ARCH_NAME = "SM100"
 SUPPORTED = "compute capability 10.x (SM100, B200)"
 
-# the reference's feature vocabulary; wk_query() knows the same names
+# the reference's feature vocabulary, then this build's own; wk_query() knows the same names
 FEATURES = (
     "gemm", "gemm_gelu", "gemm_dgelu", "gemm_accum", "gemm_fp8", "gemm_mx", "gemm_mx_out",
     "attn_fwd", "attn_bwd", "attn_fwd_fp8", "attn_bwd_fp8",
+    "rope", "qk_norm_rope",
 )
 
 _arch_of_index = {}
@@ -71,7 +72,7 @@ def supports(feature, device=None):
     """Whether ``feature`` runs on a GPU.
 
     Args:
-        feature: One of the reference's feature names (``FEATURES``).
+        feature: One of the feature names (``FEATURES``: the reference's and this build's own).
         device: CUDA device, index or tensor, or the architecture number 100. Other architecture numbers (the
             reference's 80, 86, 89, 120) are answered with ``False``: this build has kernels for 100 only.
 

@@ -1,6 +1,6 @@
 // The host side of the entry points' common case, as a CPython module (warpy_kernels_b200/_host.so).
 //
-// A call of attn_fwd, attn_bwd, gemm or quantize_mx costs 20-70 us of interpreter time when its checks, its output
+// A call of an entry point costs 20-70 us of interpreter time when its checks, its output
 // tensors and its argument block are made in Python, which is more than the kernels of a small problem take.  Here
 // the same work takes 3-6 us: arguments are read from the vectorcall array, outputs come from the caching allocator
 // without going through the dispatcher, and the C ABI entry point is called with the GIL released.
@@ -48,6 +48,9 @@ struct Abi {
   int (*gemm_mxfp8)(const wk_gemm_mx_args*, void*);
   int64_t (*gemm_mxfp8_workspace_bytes)(int, int, int);
   int (*quantize_mx)(const void*, int, int64_t, int64_t, int64_t, void*, void*, void*);
+  int (*rope)(const wk_rope_args*, void*);
+  int64_t (*qk_norm_rope_bwd_workspace_bytes)(int, int, int, int);
+  int (*qk_norm_rope_bwd)(const wk_rope_args*, void*);
 } abi;
 bool bound = false;
 
@@ -68,6 +71,9 @@ const struct {
     {"wk_gemm_mxfp8", reinterpret_cast<void**>(&abi.gemm_mxfp8)},
     {"wk_gemm_mxfp8_workspace_bytes", reinterpret_cast<void**>(&abi.gemm_mxfp8_workspace_bytes)},
     {"wk_quantize_mx", reinterpret_cast<void**>(&abi.quantize_mx)},
+    {"wk_rope", reinterpret_cast<void**>(&abi.rope)},
+    {"wk_qk_norm_rope_bwd_workspace_bytes", reinterpret_cast<void**>(&abi.qk_norm_rope_bwd_workspace_bytes)},
+    {"wk_qk_norm_rope_bwd", reinterpret_cast<void**>(&abi.qk_norm_rope_bwd)},
 };
 
 constexpr int kMaxDevices = 64;
@@ -558,6 +564,270 @@ PyObject* quantize_mx(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObje
   return r;
 }
 
+// ---- rotation of queries and keys -------------------------------------------------------------------------------
+int rope_dtype(at::ScalarType t) {
+  return t == at::kBFloat16 ? WK_BF16 : t == at::kHalf ? WK_F16 : t == at::kFloat ? WK_F32 : -1;
+}
+
+// [B, H, N, d] rows the kernels can address: last stride 1, base and other strides multiples of `unit` bytes.
+bool rope_rows(const at::Tensor& t, int64_t unit) {
+  const int64_t size = t.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (t.stride(i) * size % unit) return false;
+  return t.stride(3) == 1 && aligned(t.data_ptr(), unit);
+}
+
+// No two elements share memory: every stride spans what the smaller ones reach.
+bool apart(const at::Tensor& t) {
+  int64_t span = 1, last = 0;
+  for (;;) {  // the dimensions by their strides, smallest first
+    int next = -1, equal = 0;
+    for (int i = 0; i < 4; ++i) {
+      if (t.size(i) <= 1 || t.stride(i) <= last) continue;
+      if (next < 0 || t.stride(i) < t.stride(next)) next = i, equal = 0;
+      else if (t.stride(i) == t.stride(next)) ++equal;
+    }
+    for (int i = 0; i < 4; ++i) equal += t.size(i) > 1 && t.stride(i) <= 0;
+    if (equal) return false;
+    if (next < 0) return true;
+    if (t.stride(next) < span) return false;
+    last = t.stride(next);
+    span = last * t.size(next);
+  }
+}
+
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto bytes = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int i = 0; i < t.dim(); ++i) last += t.stride(i) * (t.size(i) - 1);
+    return (last + 1) * static_cast<int64_t>(t.element_size());
+  };
+  const char *x = static_cast<const char*>(a.data_ptr()), *y = static_cast<const char*>(b.data_ptr());
+  return x < y + bytes(b) && y < x + bytes(a);
+}
+
+// The position axis of every pair, two bits each, and the number of axes (0: positions have no axis).
+bool rope_axes(PyObject* sections, bool cycle, int64_t pairs, uint64_t (&words)[4], int64_t& axes) {
+  axes = 0;
+  if (!sections || sections == Py_None) return true;
+  if (!PyTuple_Check(sections)) return false;
+  axes = PyTuple_GET_SIZE(sections);
+  if (axes < 1 || axes > 4) return false;
+  long n[4] = {}, sum = 0;
+  for (int a = 0; a < axes; ++a) {
+    PyObject* o = PyTuple_GET_ITEM(sections, a);
+    if (!PyLong_CheckExact(o)) return false;
+    n[a] = PyLong_AsLong(o);
+    if (n[a] < 0 || n[a] > pairs) {
+      PyErr_Clear();
+      return false;
+    }
+    sum += n[a];
+    if (cycle && a && n[a] && a + axes * (n[a] - 1) >= pairs) return false;
+  }
+  if (sum != pairs) return false;
+  int a = 0;
+  for (int64_t j = 0, used = 0; j < pairs; ++j) {
+    uint64_t axis;
+    if (cycle) {
+      axis = j < axes * n[j % axes] ? j % axes : 0;
+    } else {
+      while (used == n[a]) ++a, used = 0;
+      axis = a, ++used;
+    }
+    words[j / 32] |= axis << (2 * (j % 32));
+  }
+  return true;
+}
+
+// What all rotation calls share: q, k, positions, inv_freq and how pairs are formed.
+bool rope_inputs(const at::Tensor* q, PyObject* k_obj, const at::Tensor* k, const at::Tensor* pos, const at::Tensor* freq,
+                 PyObject* sections, bool cycle, bool interleaved, wk_rope_args& a) {
+  if (!q || !pos || !freq || (!k && k_obj != Py_None) || q->dim() != 4) return false;
+  a.dtype = rope_dtype(q->scalar_type());
+  const at::Device dev = q->device();
+  if (a.dtype < 0 || !dev.is_cuda() || !device_ok(dev.index()) || !rope_rows(*q, 16)) return false;
+  const int64_t B = q->size(0), Hq = q->size(1), N = q->size(2), d = q->size(3);
+  if (B < 1 || Hq < 1 || N < 1 || B > INT32_MAX / 4 / N || Hq > (1 << 18) || d % 16 || d < 32 || d > 256) return false;
+  if (k && (k->dim() != 4 || k->size(0) != B || k->size(1) < 1 || k->size(1) > (1 << 18) || k->size(2) != N || k->size(3) != d ||
+            k->scalar_type() != q->scalar_type() || k->device() != dev || !rope_rows(*k, 16)))
+    return false;
+  const at::ScalarType ft = freq->scalar_type(), pt = pos->scalar_type();
+  if (freq->dim() != 1 || (ft != at::kFloat && ft != at::kDouble) || freq->device() != dev || !freq->is_contiguous())
+    return false;
+  const int64_t pairs = freq->size(0);
+  int64_t axes;
+  if (pairs < 8 || pairs % 8 || 2 * pairs > d || !rope_axes(sections, cycle, pairs, a.axis_map, axes)) return false;
+  if ((pt != at::kInt && pt != at::kLong) || pos->device() != dev) return false;
+  const int lead = axes ? 1 : 0;
+  const int64_t dims = pos->dim() - lead;
+  if (dims < 1 || dims > 2 || (lead && pos->size(0) != axes) || pos->size(-1) != N || (dims == 2 && pos->size(lead) != B))
+    return false;
+  a.position_strides[0] = lead ? pos->stride(0) : 0;
+  a.position_strides[1] = dims == 2 ? pos->stride(lead) : 0;
+  a.position_strides[2] = pos->stride(-1);
+  a.positions = pos->data_ptr(), a.inv_freq = freq->data_ptr();
+  a.position_int64 = pt == at::kLong, a.inv_freq_f64 = ft == at::kDouble;
+  a.interleaved = interleaved;
+  a.q = q->data_ptr(), a.k = k ? k->data_ptr() : nullptr;
+  put_strides(a.q_strides, *q);
+  if (k) put_strides(a.k_strides, *k);
+  a.B = B, a.N = N, a.Hq = Hq, a.Hk = k ? k->size(1) : 0, a.d = d, a.rot = 2 * pairs;
+  return true;
+}
+
+bool rope_weights(PyObject* q_obj, PyObject* k_obj, PyObject* eps, const at::Tensor* q, const at::Tensor* k, wk_rope_args& a) {
+  const at::Tensor *wq = tensor_of(q_obj), *wk = tensor_of(k_obj);
+  if (!wq || (k && !wk)) return false;
+  for (const at::Tensor* w : {wq, k ? wk : wq})
+    if (w->dim() != 1 || w->size(0) != a.d || w->scalar_type() != wq->scalar_type() || w->device() != q->device() ||
+        !w->is_contiguous())
+      return false;
+  a.w_dtype = rope_dtype(wq->scalar_type());
+  if (a.w_dtype < 0) return false;
+  a.q_weight = wq->data_ptr(), a.k_weight = k ? wk->data_ptr() : nullptr;
+  double e = 1e-6;
+  if (eps) {
+    if (!PyFloat_Check(eps)) return false;
+    e = PyFloat_AS_DOUBLE(eps);
+  }
+  a.eps = static_cast<float>(e);
+  return e >= 0.0;
+}
+
+at::Tensor like(const at::Tensor& x, at::ScalarType dtype) {  // the memory layout of x
+  if (x.is_non_overlapping_and_dense()) return empty_strided(x.sizes(), x.strides(), dtype, x.device());
+  return at::empty_like(x, x.options().dtype(dtype));
+}
+
+PyObject* pair_of(PyObject* a, PyObject* b) {
+  PyObject* r = PyTuple_New(2);
+  PyTuple_SET_ITEM(r, 0, a), PyTuple_SET_ITEM(r, 1, b);
+  return r;
+}
+
+PyObject* rope_forward(const at::Tensor* q, const at::Tensor* k, PyObject* q_out, PyObject* k_out,
+                       PyObject* q_descale, PyObject* k_descale, wk_rope_args& a, const char* what) {
+  auto given = [](PyObject* o) { return o && o != Py_None; };
+  const bool fp8 = given(q_descale);
+  if (given(k_descale) != (fp8 && k) || (!k && given(k_out))) return declined();
+  const at::ScalarType dtype = fp8 ? at::kFloat8_e4m3fn : q->scalar_type();
+  if (fp8) {
+    const at::Tensor *sq = tensor_of(q_descale), *sk = k ? tensor_of(k_descale) : sq;
+    for (const at::Tensor* s : {sq, sk})
+      if (!s || s->dim() != 2 || s->size(0) != a.B || s->size(1) < 1 || s->size(1) != sq->size(1) ||
+          s->scalar_type() != at::kFloat || s->device() != q->device() || !s->is_contiguous())
+        return declined();
+    a.Hkv = static_cast<int32_t>(sq->size(1));
+    if (a.Hq % a.Hkv || (k && a.Hk != a.Hkv)) return declined();
+    a.q_descale = sq->const_data_ptr<float>(), a.k_descale = k ? sk->const_data_ptr<float>() : nullptr;
+  }
+  at::Tensor outs[2];
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor* x = i ? k : q;
+    PyObject* o = i ? k_out : q_out;
+    if (!x) continue;
+    if (given(o)) {
+      const at::Tensor* t = tensor_of(o);
+      if (!t || t->dim() != 4 || t->sizes() != x->sizes() || t->scalar_type() != dtype || t->device() != x->device() ||
+          !rope_rows(*t, fp8 ? 8 : 16) || !apart(*t))
+        return declined();
+      const bool same = t->data_ptr() == x->data_ptr() && t->strides() == x->strides() && dtype == x->scalar_type();
+      if (!same && overlap(*t, *x)) return declined();
+      outs[i] = *t;
+    }
+  }
+  for (int i = 0; i < 2; ++i)
+    if ((i ? k : q) && !outs[i].defined()) outs[i] = like(i ? *k : *q, dtype);
+  a.q_out = outs[0].data_ptr();
+  put_strides(a.q_out_strides, outs[0]);
+  if (k) {
+    a.k_out = outs[1].data_ptr();
+    put_strides(a.k_out_strides, outs[1]);
+  }
+  const int code = on_device(q->device().index(), [&](void* st) { return abi.rope(&a, st); });
+  if (code) return failed(code, what);
+  return pair_of(given(q_out) ? Py_NewRef(q_out) : THPVariable_Wrap(std::move(outs[0])),
+                 !k ? Py_NewRef(Py_None) : given(k_out) ? Py_NewRef(k_out) : THPVariable_Wrap(std::move(outs[1])));
+}
+
+PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  enum { Q, K, POS, FREQ, SECTIONS, CYCLE, INTER, INVERSE, Q_OUT, K_OUT, QD, KD, COUNT };
+  static const auto names = interned<COUNT>({"q", "k", "positions", "inv_freq", "sections", "cycle", "interleaved", "inverse",
+                                             "q_out", "k_out", "q_descale", "k_descale"});
+  Params<COUNT> p;
+  bool cycle, interleaved, inverse;
+  if (!bound || !p.read(names, args, nargs, kwnames) || !p.flag(CYCLE, false, cycle) ||
+      !p.flag(INTER, false, interleaved) || !p.flag(INVERSE, false, inverse))
+    return declined();
+  const at::Tensor *q = tensor_of(p.v[Q]), *k = tensor_of(p.v[K]);
+  wk_rope_args a = {};
+  if (!rope_inputs(q, p.v[K], k, tensor_of(p.v[POS]), tensor_of(p.v[FREQ]), p.v[SECTIONS], cycle, interleaved, a))
+    return declined();
+  a.inverse = inverse;
+  return rope_forward(q, k, p.v[Q_OUT], p.v[K_OUT], p.v[QD], p.v[KD], a, "rope");
+}
+
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  enum { Q, K, WQ, WK, POS, FREQ, EPS, SECTIONS, CYCLE, INTER, Q_OUT, K_OUT, QD, KD, COUNT };
+  static const auto names = interned<COUNT>({"q", "k", "q_weight", "k_weight", "positions", "inv_freq", "eps", "sections",
+                                             "cycle", "interleaved", "q_out", "k_out", "q_descale", "k_descale"});
+  Params<COUNT> p;
+  bool cycle, interleaved;
+  if (!bound || !p.read(names, args, nargs, kwnames) || !p.flag(CYCLE, false, cycle) || !p.flag(INTER, false, interleaved))
+    return declined();
+  const at::Tensor *q = tensor_of(p.v[Q]), *k = tensor_of(p.v[K]);
+  wk_rope_args a = {};
+  if (!rope_inputs(q, p.v[K], k, tensor_of(p.v[POS]), tensor_of(p.v[FREQ]), p.v[SECTIONS], cycle, interleaved, a) ||
+      !rope_weights(p.v[WQ], p.v[WK], p.v[EPS], q, k, a))
+    return declined();
+  return rope_forward(q, k, p.v[Q_OUT], p.v[K_OUT], p.v[QD], p.v[KD], a, "qk_norm_rope");
+}
+
+PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  enum { DQ, DK, Q, K, WQ, WK, POS, FREQ, EPS, SECTIONS, CYCLE, INTER, COUNT };
+  static const auto names = interned<COUNT>({"dq_out", "dk_out", "q", "k", "q_weight", "k_weight", "positions", "inv_freq",
+                                             "eps", "sections", "cycle", "interleaved"});
+  Params<COUNT> p;
+  bool cycle, interleaved;
+  if (!bound || !p.read(names, args, nargs, kwnames) || !p.flag(CYCLE, false, cycle) || !p.flag(INTER, false, interleaved))
+    return declined();
+  const at::Tensor *q = tensor_of(p.v[Q]), *k = tensor_of(p.v[K]), *dq = tensor_of(p.v[DQ]), *dk = tensor_of(p.v[DK]);
+  wk_rope_args a = {};
+  if (!rope_inputs(q, p.v[K], k, tensor_of(p.v[POS]), tensor_of(p.v[FREQ]), p.v[SECTIONS], cycle, interleaved, a) ||
+      !rope_weights(p.v[WQ], p.v[WK], p.v[EPS], q, k, a))
+    return declined();
+  auto grad_ok = [](const at::Tensor* g, const at::Tensor& x) {
+    return g && g->dim() == 4 && g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type() && g->device() == x.device() &&
+           rope_rows(*g, 16);
+  };
+  if (!grad_ok(dq, *q) || (k ? !grad_ok(dk, *k) : p.v[DK] != Py_None)) return declined();
+  const at::Device dev = q->device();
+  const at::ScalarType wt = tensor_of(p.v[WQ])->scalar_type();
+  at::Tensor gq = like(*q, q->scalar_type()), gwq = empty({a.d}, wt, dev), gk, gwk;
+  a.dq_out = dq->data_ptr(), a.q_out = gq.data_ptr(), a.dq_weight = gwq.data_ptr();
+  put_strides(a.dq_out_strides, *dq), put_strides(a.q_out_strides, gq);
+  if (k) {
+    gk = like(*k, k->scalar_type()), gwk = empty({a.d}, wt, dev);
+    a.dk_out = dk->data_ptr(), a.k_out = gk.data_ptr(), a.dk_weight = gwk.data_ptr();
+    put_strides(a.dk_out_strides, *dk), put_strides(a.k_out_strides, gk);
+  }
+  {
+    const c10::cuda::OptionalCUDAGuard guard(dev);
+    a.workspace_bytes = abi.qk_norm_rope_bwd_workspace_bytes(a.B, a.N, a.Hq + a.Hk, a.d);
+  }
+  at::Tensor workspace = empty({a.workspace_bytes}, at::kByte, dev);
+  a.workspace = workspace.data_ptr();
+  const int code = on_device(dev.index(), [&](void* st) { return abi.qk_norm_rope_bwd(&a, st); });
+  if (code) return failed(code, "qk_norm_rope_bwd");
+  PyObject* r = PyTuple_New(4);
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(gq)));
+  PyTuple_SET_ITEM(r, 1, k ? THPVariable_Wrap(std::move(gk)) : Py_NewRef(Py_None));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(gwq)));
+  PyTuple_SET_ITEM(r, 3, k ? THPVariable_Wrap(std::move(gwk)) : Py_NewRef(Py_None));
+  return r;
+}
+
 // ---- prepared launches --------------------------------------------------------------------------------------------
 // launch(entry, args, device) -> code: calls the C ABI function at address `entry` with the argument block at address
 // `args` on the current stream of the device.
@@ -643,6 +913,9 @@ PyMethodDef methods[] = {
     {"attn_bwd", as_method<guarded<attn_bwd>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"gemm", as_method<guarded<gemm>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"quantize_mx", as_method<guarded<quantize_mx>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
+    {"rope", as_method<guarded<rope>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
+    {"qk_norm_rope", as_method<guarded<qk_norm_rope>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
+    {"qk_norm_rope_bwd", as_method<guarded<qk_norm_rope_bwd>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"launch", as_method<guarded_plain<launch>>(), METH_FASTCALL, nullptr},
     {"block_flags", as_method<guarded_plain<py_block_flags>>(), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},

@@ -186,10 +186,11 @@ extern "C" {
 int wk_query(const char* feature) {
   if (!feature) return WK_E_ARG;
   static const char* const kYes[] = {"gemm",       "gemm_fp8",   "gemm_mx",      "gemm_mx_out", "gemm_gelu",
-                                     "gemm_dgelu", "gemm_accum", "attn_fwd_fp8", "attn_bwd_fp8", "attn_fwd", "attn_bwd"};
+                                     "gemm_dgelu", "gemm_accum", "attn_fwd_fp8", "attn_bwd_fp8", "attn_fwd", "attn_bwd",
+                                     "rope",       "qk_norm_rope"};
   for (const char* f : kYes)
     if (!strcmp(f, feature)) return 1;
-  return WK_E_ARG;  // every feature name of the reference is built; anything else is not a feature
+  return WK_E_ARG;  // every feature name is built; anything else is not a feature
 }
 
 int wk_device_arch(int device) {
