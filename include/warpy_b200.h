@@ -369,6 +369,51 @@ int wk_rope(const wk_rope_args* args, void* stream);
 int64_t wk_qk_norm_rope_bwd_workspace_bytes(int B, int N, int heads, int d);
 int wk_qk_norm_rope_bwd(const wk_rope_args* args, void* stream);
 
+/* Attention of a batch of sequences over one shared prefix of keys and each sequence's own keys behind it: what
+ * wk_attn_fwd_* computes for keys and values [prefix ; own keys of the sequence], with the prefix read once for all
+ * sequences.  No counterpart in the reference.
+ *   q [B,Hq,Nq,d], k_prefix, v_prefix [1,Hkv,P,d], k, v [B,Hkv,S,d]  all e4m3 (fp8 != 0) or all bf16; strides of (B, H, N)
+ *       in elements, the last dimension contiguous, bases and strides multiples of 16 bytes.  P and S may be 0 (the
+ *       pointers are then not read)
+ *   seqused_k [B] int32 or NULL: how many of its S own keys each sequence attends to
+ *   q_descale, k_descale, v_descale [B,Hkv], k_prefix_descale, v_prefix_descale [Hkv]  fp32 contiguous, fp8 only
+ *   causal: query i of a sequence with n own keys sees the first P + n - Nq + i + 1 keys of [prefix ; own]
+ *   out [B,Hq,Nq,d] bf16, 8-byte aligned, element strides multiples of 4; lse fp32 or NULL, element strides (B, H)
+ *   workspace: wk_attn_fwd_shared_prefix_workspace_bytes, 16-byte aligned; holds nothing between calls; calls that can run
+ *       at the same time need buffers of their own
+ * Rows without a visible key get out = 0, lse = +inf.  Keys and values must be finite where a row sees them; what lies
+ * behind a sequence's last key is never used.  d 64 or 128, Hq % Hkv == 0, softmax_scale > 0. */
+typedef struct {
+  const void* q;
+  const void* k_prefix;
+  const void* v_prefix;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;
+  const float* q_descale;
+  const float* k_descale;
+  const float* v_descale;
+  const float* k_prefix_descale;
+  const float* v_prefix_descale;
+  const int32_t* seqused_k;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_strides[3];
+  int64_t k_prefix_strides[3];
+  int64_t v_prefix_strides[3];
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  int64_t out_strides[3];
+  int64_t lse_strides[2];
+  int32_t B, Hq, Hkv, Nq, P, S, d;
+  int32_t fp8, causal, lse_natural;
+  float softmax_scale;
+} wk_attn_prefix_args;
+
+int64_t wk_attn_fwd_shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int Nq, int P, int S, int d);
+int wk_attn_fwd_shared_prefix(const wk_attn_prefix_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ from warpy_kernels_b200 import arch, attn, interface, quant, rotary, utils
 from warpy_kernels_b200 import (
     attn_bwd,
     attn_fwd,
+    attn_fwd_shared_prefix,
     autotune_gemm,
     device_arch,
     gemm,

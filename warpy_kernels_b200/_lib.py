@@ -45,6 +45,8 @@ SIGNATURES = {
     "wk_rope": (_i32, [_ptr, _ptr]),
     "wk_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i32] * 4),
     "wk_qk_norm_rope_bwd": (_i32, [_ptr, _ptr]),
+    "wk_attn_fwd_shared_prefix_workspace_bytes": (_i64, [_i32] * 7),
+    "wk_attn_fwd_shared_prefix": (_i32, [_ptr, _ptr]),
 }
 
 _lib = None

@@ -18,7 +18,7 @@ SUPPORTED = "compute capability 10.x (SM100, B200)"
 FEATURES = (
     "gemm", "gemm_gelu", "gemm_dgelu", "gemm_accum", "gemm_fp8", "gemm_mx", "gemm_mx_out",
     "attn_fwd", "attn_bwd", "attn_fwd_fp8", "attn_bwd_fp8",
-    "rope", "qk_norm_rope",
+    "rope", "qk_norm_rope", "attn_fwd_shared_prefix",
 )
 
 _arch_of_index = {}

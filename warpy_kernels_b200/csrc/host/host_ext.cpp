@@ -51,6 +51,8 @@ struct Abi {
   int (*rope)(const wk_rope_args*, void*);
   int64_t (*qk_norm_rope_bwd_workspace_bytes)(int, int, int, int);
   int (*qk_norm_rope_bwd)(const wk_rope_args*, void*);
+  int64_t (*attn_prefix_workspace_bytes)(int, int, int, int, int, int, int);
+  int (*attn_prefix)(const wk_attn_prefix_args*, void*);
 } abi;
 bool bound = false;
 
@@ -74,6 +76,8 @@ const struct {
     {"wk_rope", reinterpret_cast<void**>(&abi.rope)},
     {"wk_qk_norm_rope_bwd_workspace_bytes", reinterpret_cast<void**>(&abi.qk_norm_rope_bwd_workspace_bytes)},
     {"wk_qk_norm_rope_bwd", reinterpret_cast<void**>(&abi.qk_norm_rope_bwd)},
+    {"wk_attn_fwd_shared_prefix_workspace_bytes", reinterpret_cast<void**>(&abi.attn_prefix_workspace_bytes)},
+    {"wk_attn_fwd_shared_prefix", reinterpret_cast<void**>(&abi.attn_prefix)},
 };
 
 constexpr int kMaxDevices = 64;
@@ -828,6 +832,78 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs, P
   return r;
 }
 
+PyObject* attn_fwd_shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  enum { Q, KP, VP, K, V, QD, KD, VD, KPD, VPD, CAUSAL, SCALE, OUT, LSE, USED, NATURAL, COUNT };
+  static const auto names = interned<COUNT>({"q", "k_prefix", "v_prefix", "k", "v", "q_descale", "k_descale", "v_descale",
+                                             "k_prefix_descale", "v_prefix_descale", "causal", "softmax_scale", "out",
+                                             "return_lse", "seqused_k", "lse_natural"});
+  Params<COUNT> p;
+  AttnShape s, prefix;
+  if (!bound || !p.read(names, args, nargs, kwnames)) return declined();
+  const at::Tensor *q = tensor_of(p.v[Q]), *kp = tensor_of(p.v[KP]), *vp = tensor_of(p.v[VP]);
+  const at::Tensor *k = tensor_of(p.v[K]), *v = tensor_of(p.v[V]);
+  if (!attn_shape(q, k, v, s) || !kp || !vp || kp->dim() != 4 || kp->sizes() != vp->sizes() || kp->size(0) != 1 ||
+      kp->size(1) != s.Hkv || kp->size(3) != s.d || kp->size(2) < 1 || kp->size(2) > INT32_MAX / 2)
+    return declined();
+  for (const at::Tensor* x : {kp, vp})
+    if (x->scalar_type() != q->scalar_type() || x->device() != s.dev || !tma_direct(*x)) return declined();
+  for (const at::Tensor* x : {q, kp, vp, k, v})
+    if (x->stride(0) < 1 || x->stride(1) < 1 || x->stride(2) < 1) return declined();
+  prefix = s, prefix.B = 1;
+  wk_attn_prefix_args a = {};
+  if (s.fp8) {
+    if (!descale(p.v[QD], s, a.q_descale) || !descale(p.v[KD], s, a.k_descale) || !descale(p.v[VD], s, a.v_descale) ||
+        !descale(p.v[KPD], prefix, a.k_prefix_descale) || !descale(p.v[VPD], prefix, a.v_prefix_descale))
+      return declined();
+  } else if (p.given(QD) || p.given(KD) || p.given(VD) || p.given(KPD) || p.given(VPD)) {
+    return declined();
+  }
+  bool with_lse, causal, natural;
+  if (!softmax_scale_of(p.v[SCALE], s.d, a.softmax_scale) || !p.flag(LSE, true, with_lse) ||
+      !p.flag(CAUSAL, false, causal) || !p.flag(NATURAL, false, natural))
+    return declined();
+  if (p.given(USED)) {
+    const at::Tensor* used = tensor_of(p.v[USED]);
+    if (!used || used->dim() != 1 || used->size(0) != s.B || used->scalar_type() != at::kInt || used->device() != s.dev ||
+        !used->is_contiguous())
+      return declined();
+    a.seqused_k = used->const_data_ptr<int32_t>();
+  }
+  {
+    const c10::cuda::OptionalCUDAGuard guard(s.dev);
+    a.workspace_bytes = abi.attn_prefix_workspace_bytes(s.B, s.Hq, s.Hkv, s.Nq, kp->size(2), s.Nk, s.d);
+  }
+  if (!a.workspace_bytes) return declined();
+  at::Tensor out, lse;
+  if (p.given(OUT)) {
+    const at::Tensor* o = tensor_of(p.v[OUT]);
+    if (!o || o->dim() != 4 || o->sizes() != q->sizes() || o->scalar_type() != at::kBFloat16 || o->device() != s.dev ||
+        o->stride(3) != 1 || !aligned(o->data_ptr(), 8))
+      return declined();
+    for (int i = 0; i < 3; ++i)
+      if (o->stride(i) < 1 || o->stride(i) % 4) return declined();
+    out = *o;
+  } else {
+    out = like(*q, at::kBFloat16);
+  }
+  at::Tensor workspace = empty({a.workspace_bytes}, at::kByte, s.dev);
+  if (with_lse) {
+    lse = empty({s.B, s.Hq, s.Nq}, at::kFloat, s.dev);
+    a.lse = lse.mutable_data_ptr<float>();
+    a.lse_strides[0] = s.Hq * s.Nq, a.lse_strides[1] = s.Nq;
+  }
+  a.q = q->data_ptr(), a.k_prefix = kp->data_ptr(), a.v_prefix = vp->data_ptr(), a.k = k->data_ptr(), a.v = v->data_ptr();
+  a.out = out.data_ptr(), a.workspace = workspace.data_ptr();
+  put_strides(a.q_strides, *q), put_strides(a.k_prefix_strides, *kp), put_strides(a.v_prefix_strides, *vp);
+  put_strides(a.k_strides, *k), put_strides(a.v_strides, *v), put_strides(a.out_strides, out);
+  a.B = s.B, a.Hq = s.Hq, a.Hkv = s.Hkv, a.Nq = s.Nq, a.P = kp->size(2), a.S = s.Nk, a.d = s.d;
+  a.fp8 = s.fp8, a.causal = causal, a.lse_natural = natural;
+  const int code = on_device(s.dev.index(), [&](void* st) { return abi.attn_prefix(&a, st); });
+  if (code) return failed(code, "attn_fwd_shared_prefix");
+  return pair_of(p.given(OUT) ? Py_NewRef(p.v[OUT]) : THPVariable_Wrap(std::move(out)),
+                 with_lse ? THPVariable_Wrap(std::move(lse)) : Py_NewRef(Py_None));
+}
+
 // ---- prepared launches --------------------------------------------------------------------------------------------
 // launch(entry, args, device) -> code: calls the C ABI function at address `entry` with the argument block at address
 // `args` on the current stream of the device.
@@ -916,6 +992,7 @@ PyMethodDef methods[] = {
     {"rope", as_method<guarded<rope>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"qk_norm_rope", as_method<guarded<qk_norm_rope>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"qk_norm_rope_bwd", as_method<guarded<qk_norm_rope_bwd>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
+    {"attn_fwd_shared_prefix", as_method<guarded<attn_fwd_shared_prefix>>(), METH_FASTCALL | METH_KEYWORDS, nullptr},
     {"launch", as_method<guarded_plain<launch>>(), METH_FASTCALL, nullptr},
     {"block_flags", as_method<guarded_plain<py_block_flags>>(), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},

@@ -61,9 +61,21 @@ int* status_word() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
   std::lock_guard<std::mutex> lock(g_mu);
   if (!g_status[dev]) {
+    // The first call of a process may be inside a stream capture, which neither an allocation nor work on the legacy stream
+    // may disturb.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
     int* p = nullptr;
-    if (cudaMalloc(&p, 64) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, 64) != cudaSuccess) return nullptr;
+    cudaStream_t own = nullptr;
+    const bool ok = cudaMalloc(&p, 64) == cudaSuccess &&
+                    cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(p, 0, 64, own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+    if (own) cudaStreamDestroy(own);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) {
+      if (p) cudaFree(p);
+      return nullptr;
+    }
     g_status[dev] = p;
   }
   return g_status[dev];
@@ -187,7 +199,7 @@ int wk_query(const char* feature) {
   if (!feature) return WK_E_ARG;
   static const char* const kYes[] = {"gemm",       "gemm_fp8",   "gemm_mx",      "gemm_mx_out", "gemm_gelu",
                                      "gemm_dgelu", "gemm_accum", "attn_fwd_fp8", "attn_bwd_fp8", "attn_fwd", "attn_bwd",
-                                     "rope",       "qk_norm_rope"};
+                                     "rope",       "qk_norm_rope", "attn_fwd_shared_prefix"};
   for (const char* f : kYes)
     if (!strcmp(f, feature)) return 1;
   return WK_E_ARG;  // every feature name is built; anything else is not a feature
