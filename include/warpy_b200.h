@@ -323,7 +323,7 @@ int wk_attn_bwd_bf16(const wk_attn_bwd_args* args, void* stream);
  *       e4m3 bytes.  *_strides = element strides of dims (B, H, N), the last dimension contiguous; base and strides
  *       multiples of 16 bytes (8 for e4m3 outputs).  An output may be its own input (same base and strides) but must
  *       not overlap anything else
- *   q_weight, k_weight [d]  contiguous, dtype w_dtype
+ *   q_weight, k_weight [d]  contiguous, 16-byte aligned, dtype w_dtype
  *   q_descale, k_descale    fp32 [B,Hkv] contiguous, as the FP8 attention takes them (value = code . descale);
  *       Hq % Hkv == 0, Hk == Hkv (or 0)
  *   positions [axes][B][N]  int32 or int64, element strides position_strides
@@ -365,8 +365,8 @@ typedef struct {
 int wk_rope(const wk_rope_args* args, void* stream);
 
 /* Gradients of the call above with weights: q_out, k_out receive the gradients of q and k; dq_weight, dk_weight those of
- * the weights, summed in fp32 in a fixed order.  q_descale, k_descale NULL; heads = Hq + Hk. */
-int64_t wk_qk_norm_rope_bwd_workspace_bytes(int B, int N, int heads, int d);
+ * the weights, summed in fp32 in a fixed order.  q_descale, k_descale NULL. */
+int64_t wk_qk_norm_rope_bwd_workspace_bytes(int d);
 int wk_qk_norm_rope_bwd(const wk_rope_args* args, void* stream);
 
 /* Attention of a batch of sequences over one shared prefix of keys and each sequence's own keys behind it: what

@@ -241,6 +241,8 @@ def test_gradients(cuda, B, N, Hq, Hkv, d, pairs, dtype, layout, interleaved):
     q, k, g = inputs(B, N, Hq, Hkv, d, dtype, layout)
     wt = torch.float32 if N % 2 else dtype
     wq, wk_ = weights(d, g, wt)
+    if layout == "odd":  # weights that do not start on 16 bytes
+        wq, wk_ = (torch.cat((w[:1], w))[1:] for w in (wq, wk_))
     dq, dk, _ = inputs(B, N, Hq, Hkv, d, dtype, "bhnd" if layout == "qkv" else layout, seed=5)
     pos = torch.randint(0, 5000, (B, N), device="cuda", generator=g, dtype=torch.int32)
     freq = frequencies(pairs)

@@ -43,7 +43,7 @@ SIGNATURES = {
     "wk_gemm_mxfp8_noalloc_max_bytes": (_i64, []),
     "wk_gemm_mxfp8_noalloc_status": (_i32, []),
     "wk_rope": (_i32, [_ptr, _ptr]),
-    "wk_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i32] * 4),
+    "wk_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i32]),
     "wk_qk_norm_rope_bwd": (_i32, [_ptr, _ptr]),
     "wk_attn_fwd_shared_prefix_workspace_bytes": (_i64, [_i32] * 7),
     "wk_attn_fwd_shared_prefix": (_i32, [_ptr, _ptr]),

@@ -49,7 +49,7 @@ struct Abi {
   int64_t (*gemm_mxfp8_workspace_bytes)(int, int, int);
   int (*quantize_mx)(const void*, int, int64_t, int64_t, int64_t, void*, void*, void*);
   int (*rope)(const wk_rope_args*, void*);
-  int64_t (*qk_norm_rope_bwd_workspace_bytes)(int, int, int, int);
+  int64_t (*qk_norm_rope_bwd_workspace_bytes)(int);
   int (*qk_norm_rope_bwd)(const wk_rope_args*, void*);
   int64_t (*attn_prefix_workspace_bytes)(int, int, int, int, int, int, int);
   int (*attn_prefix)(const wk_attn_prefix_args*, void*);
@@ -685,7 +685,7 @@ bool rope_weights(PyObject* q_obj, PyObject* k_obj, PyObject* eps, const at::Ten
   if (!wq || (k && !wk)) return false;
   for (const at::Tensor* w : {wq, k ? wk : wq})
     if (w->dim() != 1 || w->size(0) != a.d || w->scalar_type() != wq->scalar_type() || w->device() != q->device() ||
-        !w->is_contiguous())
+        !w->is_contiguous() || !aligned(w->data_ptr(), 16))
       return false;
   a.w_dtype = rope_dtype(wq->scalar_type());
   if (a.w_dtype < 0) return false;
@@ -818,7 +818,7 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs, P
   }
   {
     const c10::cuda::OptionalCUDAGuard guard(dev);
-    a.workspace_bytes = abi.qk_norm_rope_bwd_workspace_bytes(a.B, a.N, a.Hq + a.Hk, a.d);
+    a.workspace_bytes = abi.qk_norm_rope_bwd_workspace_bytes(a.d);
   }
   at::Tensor workspace = empty({a.workspace_bytes}, at::kByte, dev);
   a.workspace = workspace.data_ptr();

@@ -7,15 +7,23 @@
 // Backward, with g = R(-theta) dy, h = g w:
 //   dw = sum over rows of g x r     dx = r (h - x r^2 mean(h x))
 //
-// A row is d / 16 lanes of a warp with 16 elements each, two 16-byte pieces (16-bit types) that hold both halves of the
-// lane's pairs: the rotation needs no exchange, the norm one reduction over the lanes of a row.  A CTA takes all heads of
-// a few neighbouring tokens, so that an angle is made once for all heads of its token.
+// A row is d / 16 lanes of a warp with 16 elements each, two 8-element pieces that hold both halves of the lane's pairs:
+// the rotation needs no exchange, the norm one reduction over the lanes of a row.  A warp takes all heads of one token (of a
+// few, where heads are fewer than the rows it holds; a part of the heads, where tokens are few), so that an angle is made
+// once for the heads of its token and its products with the weights stay in registers.  A warp goes on to the next tokens by
+// itself; every lane fetches its own pieces a few rows ahead, across tokens, with cp.async into a ring of its own, so that
+// loads are under way while angles are made; a warp does its share of the queries, then of the keys.
 //
 // Angles: position times inv_freq in turns, reduced to half a turn in fp64 (positions beyond 2^20 leave nothing of an fp32
 // product's fraction), then sine and cosine in fp32.
 //
-// Bound by HBM: every element is read once and written once (backward: read twice).
+// Bound by HBM: every element is read once and written once (backward: read twice).  What has to be kept small for that is
+// the number of instructions: a warp's 512 elements (bf16: 2 KiB of traffic, 90 cycles at an SM's share of the bandwidth,
+// 360 issue slots of its four schedulers) take about 90.  Arithmetic goes by packed pairs of fp32.
 #include <cuda_fp16.h>
+#include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_common.h"
@@ -23,8 +31,13 @@
 namespace wk {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kCtasPerSm = 3;
 constexpr int kMaxD = 256;
+// Rows of a warp that are under way: 16-bit types 6 KiB a warp and 96 KiB an SM forward, half again as many bytes otherwise.
+template <typename T, bool BWD>
+constexpr int kStages = sizeof(T) == 2 ? (BWD ? 4 : 6) : (BWD ? 3 : 4);
+constexpr int kTable = 512;  // cosines and sines of a warp's tokens: at most 32 rows / LPR . 8 LPR pairs
 
 struct RopeParams {
   const void* x[2];  // queries, keys
@@ -37,312 +50,545 @@ struct RopeParams {
   float* partial;  // backward: [CTA][2][d]
   int64_t xs[2][3], ys[2][3], dys[2][3], ps[3];
   uint64_t axis_map[4];
-  int B, N, Hq, H;  // H: heads of queries and keys
-  int tokens, per_cta;
+  int heads[2];
+  int N, tokens;
   int d, rot;
-  int group;  // query heads per descale entry
-  int hkv;
+  int hkv;          // descale entries per batch item
+  float inv_group;  // of the query heads that share one
+  int hb, tb;       // heads and tokens that a warp holds at a time
+  int hs;           // warps that share the heads of a token
   int w_dtype, pos64, freq64, interleaved, inverse;
   float eps;
 };
 
+// A lane's 16 elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v);
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
-  const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float* v) {
-  const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f16x2_to_float2(w[i], v[2 * i], v[2 * i + 1]);
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* v) {
-  const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* v) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                            pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(__half* p, const float* v) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void store8(float* p, const float* v) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(uint8_t* p, const float* v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7]));
-}
-
-__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
-  if (dtype == WK_F32) return static_cast<const float*>(w)[i];
-  if (dtype == WK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
-  return __half2float(static_cast<const __half*>(w)[i]);
-}
-
-// Cosine and sine of a CTA's tokens: cos at [token][pair], sin behind them.
-__device__ __forceinline__ void make_table(const RopeParams& p, int t0, int nt, float* table) {
-  const int h = p.rot / 2;
-  for (int i = threadIdx.x; i < nt * h; i += kThreads) {
-    const int t = i / h, j = i - t * h;
-    const int axis = static_cast<int>(p.axis_map[j >> 5] >> (2 * (j & 31))) & 3;
-    const int b = (t0 + t) / p.N, n = (t0 + t) - b * p.N;
-    const int64_t at = axis * p.ps[0] + b * p.ps[1] + n * p.ps[2];
-    const double pos = p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[at])
-                               : static_cast<double>(static_cast<const int32_t*>(p.positions)[at]);
-    const double f = p.freq64 ? static_cast<const double*>(p.inv_freq)[j]
-                              : static_cast<double>(static_cast<const float*>(p.inv_freq)[j]);
-    const double turns = pos * (f * 0.15915494309189533577);  // 1 / (2 pi)
-    const float rest = static_cast<float>(turns - rint(turns));
-    float s, c;
-    sincospif(2.f * rest, &s, &c);
-    table[i] = c;
-    table[p.per_cta * h + i] = p.inverse ? -s : s;
-  }
-}
-
-// The two 8-element pieces of a lane: both members of its pairs.
-__device__ __forceinline__ void pieces(const RopeParams& p, int lane, int& a, int& b) {
-  const int half = p.rot / 16;
-  if (p.interleaved || lane >= half) {
-    a = 16 * lane, b = a + 8;
-  } else {
-    a = 8 * lane, b = a + p.rot / 2;
-  }
-}
-
-// Turns the pairs of a lane's 16 values; sign -1 turns them back.
-__device__ __forceinline__ void turn(float (&v)[16], const float* cos, const float* sin, bool interleaved, float sign) {
-  float c[8], s[8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float4 x = reinterpret_cast<const float4*>(cos)[i], y = reinterpret_cast<const float4*>(sin)[i];
-    c[4 * i] = x.x, c[4 * i + 1] = x.y, c[4 * i + 2] = x.z, c[4 * i + 3] = x.w;
-    s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
-  }
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = v[2 * i], y = v[2 * i + 1], sn = sign * s[i];
-      v[2 * i] = x * c[i] - y * sn;
-      v[2 * i + 1] = y * c[i] + x * sn;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = v[i], y = v[8 + i], sn = sign * s[i];
-      v[i] = x * c[i] - y * sn;
-      v[8 + i] = y * c[i] + x * sn;
-    }
-  }
-}
-
-// Where a row is: its token in the CTA, and whether it is a query's or a key's head.
-struct Row {
-  int t, which, head, b, n;
+struct Raw {
+  uint4 a, b;
 };
-__device__ __forceinline__ Row row_at(const RopeParams& p, int t0, int row) {
-  Row r;
-  r.t = row / p.H;
-  const int h = row - r.t * p.H;
-  r.which = h >= p.Hq;
-  r.head = r.which ? h - p.Hq : h;
-  r.b = (t0 + r.t) / p.N;
-  r.n = (t0 + r.t) - r.b * p.N;
-  return r;
+template <>
+struct Raw<float> {
+  float4 a0, a1, b0, b1;
+};
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ int64_t offset(const int64_t (&s)[3], const Row& r) {
-  return r.b * s[0] + r.head * s[1] + r.n * s[2];
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
-
-template <int LPR>
-__device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-  for (int i = LPR / 2; i > 0; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-  return x;
-}
-
-// LPR: lanes of a row, at least d / 16.
-template <typename T, bool FP8, bool NORM, int LPR>
-__global__ void __launch_bounds__(kThreads)
-rope_kernel(const __grid_constant__ RopeParams p) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int SLOTS = kThreads / LPR;
-  float* weights = smem;  // [2][d]
-  float* table = smem + (NORM ? 2 * p.d : 0);
-  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-  const int t0 = blockIdx.x * p.per_cta, nt = min(p.per_cta, p.tokens - t0);
-  const int rows = nt * p.H, h = p.rot / 2;
-  const bool mine = lane < p.d / 16;
-  const bool turned = lane < p.rot / 16;
-  int at_a, at_b;
-  pieces(p, lane, at_a, at_b);
-  pdl_launch_dependents();
-  pdl_wait();
-
-  auto load = [&](const Row& r, float (&v)[16]) {
-    const T* src = static_cast<const T*>(p.x[r.which]) + offset(p.xs[r.which], r);
-    load8<T>(src + at_a, v);
-    load8<T>(src + at_b, v + 8);
-  };
-  float v[16];
-  Row r = {};
-  bool live = mine && slot < rows;
-  if (live) {  // under way while the angles are made
-    r = row_at(p, t0, slot);
-    load(r, v);
+// A warp's 512 elements in the ring: 16-byte pieces, lane after lane.
+template <typename T>
+constexpr int kRowBytes = 512 * sizeof(T);
+template <typename T>
+__device__ __forceinline__ void fetch_raw(uint32_t dst, const T* p, int at_a, int at_b) {
+  cp_async16(dst, p + at_a);
+  cp_async16(dst + 512, p + at_b);
+  if (sizeof(T) == 4) {
+    cp_async16(dst + 1024, p + at_a + 4);
+    cp_async16(dst + 1536, p + at_b + 4);
   }
-  make_table(p, t0, nt, table);
-  if (NORM)
-    for (int i = threadIdx.x; i < 2 * p.d; i += kThreads)
-      weights[i] = i < p.d ? weight_at(p.w[0], p.w_dtype, i) : p.x[1] ? weight_at(p.w[1], p.w_dtype, i - p.d) : 0.f;
-  __syncthreads();
+}
+template <typename T>
+__device__ __forceinline__ void read_raw(uint32_t src, Raw<T>& r) {
+  r.a = lds128(src), r.b = lds128(src + 512);
+}
+__device__ __forceinline__ void read_raw(uint32_t src, Raw<float>& r) {
+  auto f = [](uint4 w) {
+    return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+  };
+  r.a0 = f(lds128(src)), r.b0 = f(lds128(src + 512)), r.a1 = f(lds128(src + 1024)), r.b1 = f(lds128(src + 1536));
+}
+__device__ __forceinline__ uint64_t widen(uint32_t w, __nv_bfloat16) {
+  return pack_f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint64_t widen(uint32_t w, __half) {
+  float lo, hi;
+  f16x2_to_float2(w, lo, hi);
+  return pack_f32x2(lo, hi);
+}
+// As eight pairs of fp32, the first piece's four first.
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, uint64_t (&v)[8]) {
+  v[0] = widen(r.a.x, T()), v[1] = widen(r.a.y, T()), v[2] = widen(r.a.z, T()), v[3] = widen(r.a.w, T());
+  v[4] = widen(r.b.x, T()), v[5] = widen(r.b.y, T()), v[6] = widen(r.b.z, T()), v[7] = widen(r.b.w, T());
+}
+__device__ __forceinline__ void unpack(const Raw<float>& r, uint64_t (&v)[8]) {
+  v[0] = pack_f32x2(r.a0.x, r.a0.y), v[1] = pack_f32x2(r.a0.z, r.a0.w);
+  v[2] = pack_f32x2(r.a1.x, r.a1.y), v[3] = pack_f32x2(r.a1.z, r.a1.w);
+  v[4] = pack_f32x2(r.b0.x, r.b0.y), v[5] = pack_f32x2(r.b0.z, r.b0.w);
+  v[6] = pack_f32x2(r.b1.x, r.b1.y), v[7] = pack_f32x2(r.b1.z, r.b1.w);
+}
 
-  for (int row = slot;; row += SLOTS) {
-    if (NORM) {
-      float ss = 0.f;
-      if (live) {
+__device__ __forceinline__ uint32_t narrow(uint64_t v, __nv_bfloat16) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ uint32_t narrow(uint64_t v, __half) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  uint32_t w;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  return w;
+}
+// Four pairs to memory.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const uint64_t* v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(narrow(v[0], T()), narrow(v[1], T()), narrow(v[2], T()), narrow(v[3], T()));
+}
+__device__ __forceinline__ void store8(float* p, const uint64_t* v) {
+  float f[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(v[i], v[i], ss);
+  for (int i = 0; i < 4; ++i) unpack_f32x2(v[i], f[2 * i], f[2 * i + 1]);
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store8(uint8_t* p, const uint64_t* v) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack_f32x2(v[i], f[2 * i], f[2 * i + 1]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
+}
+
+// Eight elements of a weight, 16-byte aligned like the pieces.
+__device__ __forceinline__ void weight8(const void* w, int dtype, int at, float* v) {
+  if (dtype == WK_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
+    const float4 a = p[0], b = p[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + at);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t y = dtype == WK_BF16 ? widen(x[i], __nv_bfloat16()) : widen(x[i], __half());
+      unpack_f32x2(y, v[2 * i], v[2 * i + 1]);
+    }
+  }
+}
+
+// What a lane is in its warp.  LPR: lanes of a row where that is a power of two (0: any number).
+template <int LPR>
+struct Place {
+  int lpr, in_row, hslot, tslot;
+  int at_a, at_b;  // its two pieces
+  bool active, turned;
+  __device__ __forceinline__ explicit Place(const RopeParams& p) {
+    const int lane = threadIdx.x % 32;
+    lpr = LPR ? LPR : p.d / 16;
+    const int slot = lane / lpr;
+    in_row = lane - slot * lpr;
+    tslot = slot / p.hb, hslot = slot - tslot * p.hb;
+    active = tslot < p.tb;
+    turned = in_row < p.rot / 16;
+    if (p.interleaved || !turned) {
+      at_a = 16 * in_row, at_b = at_a + 8;
+    } else {
+      at_a = 8 * in_row, at_b = at_a + p.rot / 2;
+    }
+  }
+  __device__ __forceinline__ float row_sum(float x) const {
+    if (LPR) {
+#pragma unroll
+      for (int i = LPR / 2; i > 0; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+      return x;
+    }
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int i = 8; i > 0; i >>= 1) {
+      const float y = __shfl_down_sync(0xffffffffu, x, i);
+      if (in_row < i && in_row + i < lpr) x += y;
+    }
+    return __shfl_sync(0xffffffffu, x, lane - in_row);
+  }
+};
+
+// The lane's cosines and sines of its token.  The lanes of a token divide its pairs and exchange them in `table`
+// ([token of the warp][cos, sin][pair]).
+template <typename T, int LPR>
+__device__ __forceinline__ void angles(const RopeParams& p, const Place<LPR>& at, bool live, int b, int n, float* table,
+                                       float (&c)[8], float (&s)[8]) {
+  const int pairs = p.rot / 2;
+  float* mine = table + at.tslot * 2 * pairs;
+  if (live) {
+    const int every = p.hb * at.lpr;
+    for (int j0 = at.hslot * at.lpr + at.in_row; j0 < pairs; j0 += 2 * every) {
+      double turns[2];  // two at a time: their loads go together
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = min(j0 + i * every, pairs - 1);
+        const int axis = static_cast<int>(p.axis_map[j >> 5] >> (2 * (j & 31))) & 3;
+        const int64_t from = axis * p.ps[0] + b * p.ps[1] + n * p.ps[2];
+        const double pos = p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[from])
+                                   : static_cast<double>(static_cast<const int32_t*>(p.positions)[from]);
+        const double f = p.freq64 ? static_cast<const double*>(p.inv_freq)[j]
+                                  : static_cast<double>(static_cast<const float*>(p.inv_freq)[j]);
+        turns[i] = pos * (f * 0.15915494309189533577);  // 1 / (2 pi)
       }
-      ss = row_sum<LPR>(ss);
-      if (live) {
-        const float f = rsqrtf(ss / static_cast<float>(p.d) + p.eps);
-        const float* w = weights + r.which * p.d;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] *= f * w[at_a + i];
-          v[8 + i] *= f * w[at_b + i];
+      for (int i = 0; i < 2; ++i) {
+        const int j = j0 + i * every;
+        float sn, cs;
+        const float rest = static_cast<float>(turns[i] - rint(turns[i]));
+        if (sizeof(T) == 4) {
+          sincospif(2.f * rest, &sn, &cs);
+        } else {  // 2^-21 off within half a turn, which 16 bits of output do not see; a quarter of the instructions
+          __sincosf(6.2831853071795865f * rest, &sn, &cs);
+        }
+        if (j < pairs) {
+          mine[j] = cs;
+          mine[pairs + j] = p.inverse ? -sn : sn;
         }
       }
     }
-    if (live) {
-      if (turned) turn(v, table + r.t * h + 8 * lane, table + (p.per_cta + r.t) * h + 8 * lane, p.interleaved, 1.f);
-      if (FP8) {
-        const float inv = 1.f / p.descale[r.which][r.b * p.hkv + (r.which ? r.head : r.head / p.group)];
+  }
+  __syncwarp();
+  if (live && at.turned) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= inv;
-        uint8_t* dst = static_cast<uint8_t*>(p.y[r.which]) + offset(p.ys[r.which], r);
-        store8(dst + at_a, v);
-        store8(dst + at_b, v + 8);
-      } else {
-        T* dst = static_cast<T*>(p.y[r.which]) + offset(p.ys[r.which], r);
-        store8(dst + at_a, v);
-        store8(dst + at_b, v + 8);
+    for (int i = 0; i < 2; ++i) {
+      const float4 x = reinterpret_cast<const float4*>(mine + 8 * at.in_row)[i];
+      const float4 y = reinterpret_cast<const float4*>(mine + pairs + 8 * at.in_row)[i];
+      c[4 * i] = x.x, c[4 * i + 1] = x.y, c[4 * i + 2] = x.z, c[4 * i + 3] = x.w;
+      s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
+    }
+  }
+  __syncwarp();  // the table may be written again
+}
+
+// Rotation of a lane's values with factors folded in: y[i] = v[i] own[i] + (the other member of each pair) other[i].
+__device__ __forceinline__ uint64_t swapped(uint64_t v) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return pack_f32x2(hi, lo);
+}
+__device__ __forceinline__ void turn(const uint64_t (&v)[8], const uint64_t (&own)[8], const uint64_t (&other)[8], bool turned,
+                                     bool interleaved, uint64_t (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = mul_f32x2(v[i], own[i]);
+  if (turned) {
+    if (interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fma_f32x2(swapped(v[i]), other[i], y[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = fma_f32x2(v[i ^ 4], other[i], y[i]);
+    }
+  }
+}
+// The factors, from cosines, sines and the weights of the value that is multiplied.
+__device__ __forceinline__ void factors(const float (&c)[8], const float (&s)[8], const float (&w)[16], bool turned, bool interleaved,
+                                        uint64_t (&own)[8], uint64_t (&other)[8]) {
+  if (!turned) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own[i] = pack_f32x2(w[2 * i], w[2 * i + 1]), other[i] = 0;
+  } else if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      own[i] = pack_f32x2(c[i] * w[2 * i], c[i] * w[2 * i + 1]);
+      other[i] = pack_f32x2(-s[i] * w[2 * i + 1], s[i] * w[2 * i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      own[i] = pack_f32x2(c[2 * i] * w[2 * i], c[2 * i + 1] * w[2 * i + 1]);
+      own[4 + i] = pack_f32x2(c[2 * i] * w[8 + 2 * i], c[2 * i + 1] * w[9 + 2 * i]);
+      other[i] = pack_f32x2(-s[2 * i] * w[8 + 2 * i], -s[2 * i + 1] * w[9 + 2 * i]);
+      other[4 + i] = pack_f32x2(s[2 * i] * w[2 * i], s[2 * i + 1] * w[2 * i + 1]);
+    }
+  }
+}
+
+// The rotation alone, backwards: cosines and sines as they are, which takes half the registers.
+__device__ __forceinline__ void turn_back(const uint64_t (&v)[8], const float (&c)[8], const float (&s)[8], bool turned,
+                                          bool interleaved, uint64_t (&y)[8]) {
+  if (!turned) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[i];
+  } else if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float a, b;
+      unpack_f32x2(v[i], a, b);
+      y[i] = pack_f32x2(a * c[i] + b * s[i], b * c[i] - a * s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t c2 = pack_f32x2(c[2 * i], c[2 * i + 1]), s2 = pack_f32x2(s[2 * i], s[2 * i + 1]);
+      y[i] = fma_f32x2(v[4 + i], s2, mul_f32x2(v[i], c2));
+      y[4 + i] = fma_f32x2(mul_f32x2(v[i], s2), pack_f32x2(-1.f, -1.f), mul_f32x2(v[4 + i], c2));
+    }
+  }
+}
+
+__device__ __forceinline__ float sum_of(uint64_t v) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ float dot(const uint64_t (&a)[8], const uint64_t (&b)[8]) {
+  uint64_t x = mul_f32x2(a[0], b[0]), y = mul_f32x2(a[4], b[4]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) x = fma_f32x2(a[i], b[i], x), y = fma_f32x2(a[4 + i], b[4 + i], y);
+  return sum_of(add_f32x2(x, y));
+}
+
+// The groups of tokens that a warp works through, first for the queries, then for the keys; it takes one of the `hs` shares
+// of their heads.  hs divides the number of warps, so that neither the share nor the distance to the next group changes, and
+// the keys' groups go round from where the queries' ended.
+template <int LPR>
+struct Walk {
+  int side, group, groups, group_step;
+  int token, b, n, token_step, b_step, n_step;  // of this lane
+  __device__ __forceinline__ Walk(const RopeParams& p, const Place<LPR>& at) {
+    group_step = gridDim.x * (kThreads / 32) / p.hs;
+    groups = (p.tokens + p.tb - 1) / p.tb;
+    token_step = group_step * p.tb;
+    b_step = token_step / p.N, n_step = token_step - b_step * p.N;
+    begin(p, at, 0);
+  }
+  __device__ __forceinline__ void begin(const RopeParams& p, const Place<LPR>& at, int which) {
+    side = which;
+    group = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) / p.hs;
+    if (side) {
+      const int behind = groups % group_step;
+      group += group < behind ? group_step - behind : -behind;
+    }
+    token = group * p.tb + at.tslot;
+    b = token / p.N, n = token - b * p.N;
+  }
+  __device__ __forceinline__ bool here() const { return group < groups; }
+  __device__ __forceinline__ void next(const RopeParams& p) {
+    group += group_step, token += token_step, b += b_step, n += n_step;
+    if (n >= p.N) n -= p.N, ++b;
+  }
+};
+
+// The rows that a lane fetches ahead into its ring: IN tensors (backward: also the gradients).
+template <typename T, int LPR, bool BWD>
+struct Fetcher {
+  static constexpr int IN = BWD ? 2 : 1, STAGES = kStages<T, BWD>, BYTES = IN * kRowBytes<T>;
+  Walk<LPR> walk;
+  uint32_t ring;
+  int h, first, every, heads;
+  const T* from[IN];
+  int64_t step[IN];
+  __device__ __forceinline__ Fetcher(const RopeParams& p, const Place<LPR>& at, uint32_t ring, int first, int every)
+      : walk(p, at), ring(ring), first(first), every(every) {
+    side(p, 0);
+    if (!walk.here()) go_on(p, at);
+  }
+  __device__ __forceinline__ void side(const RopeParams& p, int which) {
+    heads = p.heads[which];
+    step[0] = every * p.xs[which][1];
+    if (BWD) step[IN - 1] = every * p.dys[which][1];
+    start(p);
+  }
+  __device__ __forceinline__ void start(const RopeParams& p) {
+    const int w = walk.side;
+    h = first;
+    from[0] = static_cast<const T*>(p.x[w]) + walk.b * p.xs[w][0] + walk.n * p.xs[w][2] + first * p.xs[w][1];
+    if (BWD)
+      from[IN - 1] = static_cast<const T*>(p.dy[w]) + walk.b * p.dys[w][0] + walk.n * p.dys[w][2] + first * p.dys[w][1];
+  }
+  // To the keys, once the queries are through.
+  __device__ __forceinline__ void go_on(const RopeParams& p, const Place<LPR>& at) {
+    if (walk.side || !p.heads[1]) return;
+    walk.begin(p, at, 1);
+    side(p, 1);
+  }
+  __device__ __forceinline__ void operator()(const RopeParams& p, const Place<LPR>& at, int stage) {
+    if (walk.here()) {
+      if (at.active && walk.token < p.tokens && h < heads) {
+#pragma unroll
+        for (int i = 0; i < IN; ++i) fetch_raw(ring + stage * BYTES + i * kRowBytes<T>, from[i], at.at_a, at.at_b);
+      }
+      h += every;
+#pragma unroll
+      for (int i = 0; i < IN; ++i) from[i] += step[i];
+      if (h - at.hslot >= heads) {  // the same for the whole warp
+        walk.next(p);
+        if (walk.here()) start(p);
+        else go_on(p, at);
       }
     }
-    if ((row - slot) + SLOTS >= rows) break;  // the same for the whole CTA: the reduction above takes whole warps
-    live = mine && row + SLOTS < rows;
-    if (live) {
-      r = row_at(p, t0, row + SLOTS);
-      load(r, v);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+};
+
+template <typename T, bool FP8, bool NORM, int LPR>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+rope_kernel(const __grid_constant__ RopeParams p) {
+  using Out = typename std::conditional<FP8, uint8_t, T>::type;
+  using Fetch = Fetcher<T, LPR, false>;
+  constexpr int WARPS = kThreads / 32;
+  extern __shared__ __align__(16) uint8_t ring_mem[];
+  __shared__ __align__(16) float tables[WARPS][kTable];
+  const int warp = threadIdx.x / 32;
+  const uint32_t ring = smem_u32(ring_mem) + warp * Fetch::STAGES * Fetch::BYTES + (threadIdx.x % 32) * 16;
+  const Place<LPR> at(p);
+  const float inv_d = 1.f / static_cast<float>(p.d);
+  const int first = (blockIdx.x * WARPS + warp) % p.hs * p.hb + at.hslot, every = p.hs * p.hb;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  Fetch fetch(p, at, ring, first, every);
+  for (int i = 0; i < Fetch::STAGES; ++i) fetch(p, at, i);
+  int stage = 0;
+  Walk<LPR> now(p, at);
+  for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
+    if (side) now.begin(p, at, 1);
+    const int heads = p.heads[side];
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 1.f;
+    if (NORM && at.active && now.here()) {
+      weight8(p.w[side], p.w_dtype, at.at_a, w);
+      weight8(p.w[side], p.w_dtype, at.at_b, w + 8);
+    }
+    const int64_t to_step = every * p.ys[side][1];
+    for (; now.here(); now.next(p)) {
+      const bool live = at.active && now.token < p.tokens;
+      uint64_t own[8], other[8];
+      {
+        float c[8], s[8];
+        angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
+        factors(c, s, w, at.turned, p.interleaved, own, other);
+      }
+      Out* to = static_cast<Out*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
+      for (int h = first; h - at.hslot < heads; h += every, to += to_step) {
+        const bool row = live && h < heads;
+        float scale = 1.f;
+        if (FP8 && row)  // h / group, exact: heads are fewer than 2^20
+          scale = p.descale[side][now.b * p.hkv + (side ? h : static_cast<int>((static_cast<float>(h) + 0.5f) * p.inv_group))];
+        asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
+        uint64_t v[8], y[8];
+        {
+          Raw<T> raw;
+          read_raw(ring + stage * Fetch::BYTES, raw);
+          unpack(raw, v);
+        }
+        float f = 1.f;
+        if (NORM) f = rsqrtf(at.row_sum(dot(v, v)) * inv_d + p.eps);
+        turn(v, own, other, at.turned, p.interleaved, y);
+        if (FP8) f *= __frcp_rn(scale);
+        if (NORM || FP8) {
+          const uint64_t f2 = pack_f32x2(f, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = mul_f32x2(y[i], f2);
+        }
+        if (row) {
+          store8(to + at.at_a, y);
+          store8(to + at.at_b, y + 4);
+        }
+        fetch(p, at, stage);  // into the place that has just been read
+        if (++stage == Fetch::STAGES) stage = 0;
+      }
     }
   }
 }
 
 template <typename T, int LPR>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
 norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int SLOTS = kThreads / LPR, WARPS = kThreads / 32;
-  float* weights = smem;  // [2][d]
-  float* table = smem + 2 * p.d;
-  const int lane = threadIdx.x % LPR, slot = threadIdx.x / LPR;
-  const int h = p.rot / 2;
-  const bool mine = lane < p.d / 16;
-  const bool turned = lane < p.rot / 16;
-  int at_a, at_b;
-  pieces(p, lane, at_a, at_b);
+  using Fetch = Fetcher<T, LPR, true>;
+  constexpr int WARPS = kThreads / 32;
+  extern __shared__ __align__(16) uint8_t ring_mem[];
+  __shared__ __align__(16) float tables[WARPS][kTable];
+  __shared__ float sums[2][WARPS][kMaxD];
+  const int warp = threadIdx.x / 32;
+  const uint32_t ring = smem_u32(ring_mem) + warp * Fetch::STAGES * Fetch::BYTES + (threadIdx.x % 32) * 16;
+  const Place<LPR> at(p);
+  const float inv_d = 1.f / static_cast<float>(p.d);
+  const int first = (blockIdx.x * WARPS + warp) % p.hs * p.hb + at.hslot, every = p.hs * p.hb;
   pdl_launch_dependents();
   pdl_wait();
-  for (int i = threadIdx.x; i < 2 * p.d; i += kThreads)
-    weights[i] = i < p.d ? weight_at(p.w[0], p.w_dtype, i) : p.x[1] ? weight_at(p.w[1], p.w_dtype, i - p.d) : 0.f;
 
-  float dw[2][16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-
-  for (int t0 = blockIdx.x * p.per_cta; t0 < p.tokens; t0 += gridDim.x * p.per_cta) {
-    const int nt = min(p.per_cta, p.tokens - t0), rows = nt * p.H;
-    __syncthreads();  // the table of the tokens before has been read
-    make_table(p, t0, nt, table);
-    __syncthreads();
-    for (int row0 = 0; row0 < rows; row0 += SLOTS) {
-      const bool live = mine && row0 + slot < rows;
-      Row r = {};
-      float x[16], g[16];
-      float ss = 0.f, hx = 0.f;
-      if (live) {
-        r = row_at(p, t0, row0 + slot);
-        const T* xp = static_cast<const T*>(p.x[r.which]) + offset(p.xs[r.which], r);
-        const T* gp = static_cast<const T*>(p.dy[r.which]) + offset(p.dys[r.which], r);
-        load8<T>(xp + at_a, x);
-        load8<T>(xp + at_b, x + 8);
-        load8<T>(gp + at_a, g);
-        load8<T>(gp + at_b, g + 8);
-        if (turned) turn(g, table + r.t * h + 8 * lane, table + (p.per_cta + r.t) * h + 8 * lane, p.interleaved, -1.f);
-        const float* w = weights + r.which * p.d;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          ss = fmaf(x[i], x[i], ss);
-          hx = fmaf(g[i] * w[i < 8 ? at_a + i : at_b + i - 8], x[i], hx);
-        }
+  Fetch fetch(p, at, ring, first, every);
+  for (int i = 0; i < Fetch::STAGES; ++i) fetch(p, at, i);
+  int stage = 0;
+  Walk<LPR> now(p, at);
+  for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
+    if (side) now.begin(p, at, 1);
+    const int heads = p.heads[side];
+    uint64_t w[8], dw[8];
+    {
+      float v[16] = {};
+      if (at.active) {
+        weight8(p.w[side], p.w_dtype, at.at_a, v);
+        weight8(p.w[side], p.w_dtype, at.at_b, v + 8);
       }
-      ss = row_sum<LPR>(ss);
-      hx = row_sum<LPR>(hx);
-      if (live) {
-        const float inv_d = 1.f / static_cast<float>(p.d);
-        const float f = rsqrtf(ss * inv_d + p.eps);
-        const float m = f * f * hx * inv_d;
-        const float* w = weights + r.which * p.d;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float gx = g[i] * x[i] * f;
-          dw[0][i] += r.which ? 0.f : gx;
-          dw[1][i] += r.which ? gx : 0.f;
-          x[i] = f * (g[i] * w[i < 8 ? at_a + i : at_b + i - 8] - x[i] * m);
+      for (int i = 0; i < 8; ++i) w[i] = pack_f32x2(v[2 * i], v[2 * i + 1]), dw[i] = 0;
+    }
+    const int64_t to_step = every * p.ys[side][1];
+    for (; now.here(); now.next(p)) {
+      const bool live = at.active && now.token < p.tokens;
+      float c[8], s[8];
+      angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
+      T* to = static_cast<T*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
+      for (int head = first; head - at.hslot < heads; head += every, to += to_step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
+        uint64_t x[8], g[8], h[8];
+        {
+          Raw<T> raw;
+          uint64_t dy[8];
+          read_raw(ring + stage * Fetch::BYTES + kRowBytes<T>, raw);
+          unpack(raw, dy);
+          turn_back(dy, c, s, at.turned, p.interleaved, g);
+          read_raw(ring + stage * Fetch::BYTES, raw);
+          unpack(raw, x);
         }
-        T* dst = static_cast<T*>(p.y[r.which]) + offset(p.ys[r.which], r);
-        store8(dst + at_a, x);
-        store8(dst + at_b, x + 8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = mul_f32x2(g[i], w[i]);
+        const float ss = at.row_sum(dot(x, x)), hx = at.row_sum(dot(h, x));
+        const float f = rsqrtf(ss * inv_d + p.eps), m = -f * f * f * hx * inv_d;
+        const uint64_t f2 = pack_f32x2(f, f), m2 = pack_f32x2(m, m);
+        if (live && head < heads) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dw[i] = fma_f32x2(mul_f32x2(g[i], x[i]), f2, dw[i]);
+            h[i] = fma_f32x2(x[i], m2, mul_f32x2(h[i], f2));
+          }
+          store8(to + at.at_a, h);
+          store8(to + at.at_b, h + 4);
+        }
+        fetch(p, at, stage);
+        if (++stage == Fetch::STAGES) stage = 0;
+      }
+    }
+    // the weight's gradient over the rows of the warp
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v[2];
+      unpack_f32x2(dw[i], v[0], v[1]);
+      const int e = i < 4 ? at.at_a + 2 * i : at.at_b + 2 * (i - 4);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = v[j];
+        if (LPR) {
+#pragma unroll
+          for (int o = 16; o >= LPR; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        } else {
+          for (int o = at.lpr; o + at.lpr <= 32; o += at.lpr) {
+            const float other = __shfl_down_sync(0xffffffffu, v[j], o);
+            if (threadIdx.x % 32 < at.lpr) sum += other;
+          }
+        }
+        if (threadIdx.x % 32 < at.lpr) sums[side][warp][e + j] = sum;
       }
     }
   }
-
-  // the weights' gradients of this CTA: over the rows of a warp, then over the warps, always in the same order
+  // and over the warps, always in the same order
   __syncthreads();
-  float* sums = smem;  // [WARPS][d], for queries and then for keys
+  for (int i = threadIdx.x; i < (p.heads[1] ? 2 : 1) * p.d; i += kThreads) {
+    const int side = i >= p.d, e = side ? i - p.d : i;
+    float sum = 0.f;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-#pragma unroll
-      for (int o = 16; o >= LPR; o >>= 1) dw[q][i] += __shfl_xor_sync(0xffffffffu, dw[q][i], o);
-      if (threadIdx.x % 32 < LPR && mine) sums[(threadIdx.x / 32) * p.d + (i < 8 ? at_a + i : at_b + i - 8)] = dw[q][i];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.d; i += kThreads) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) s += sums[w * p.d + i];
-      p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + q) * p.d + i] = s;
-    }
-    __syncthreads();
+    for (int v = 0; v < WARPS; ++v) sum += sums[side][v][e];
+    p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + side) * p.d + e] = sum;
   }
 }
 
@@ -371,20 +617,29 @@ dweight_kernel(const float* __restrict__ partial, int parts, int d, void* dw_q, 
     static_cast<__half*>(out)[col] = __float2half_rn(s);
 }
 
-int lanes_of(int d) { return d <= 32 ? 2 : d <= 64 ? 4 : d <= 128 ? 8 : 16; }
-
-// Tokens of a CTA: four passes over its rows, fewer where the tokens would not fill the SMs.
-int tokens_per_cta(int64_t tokens, int heads, int d, int sms) {
-  const int slots = kThreads / lanes_of(d);
-  int n = 4 * slots / heads;
-  const int64_t share = (tokens + 4 * sms - 1) / (4 * sms);
-  if (n > share) n = static_cast<int>(share);
-  return n < 1 ? 1 : n > 16 ? 16 : n;
-}
-
-int bwd_ctas(int64_t tokens, int per_cta, int sms) {
-  const int64_t groups = (tokens + per_cta - 1) / per_cta, most = 3ll * sms;
-  return static_cast<int>(groups < most ? groups : most);
+// How a warp's rows are divided into heads and tokens: the division that takes the fewest instructions per token (100 for a
+// step over its rows, 40 for an angle, 60 for a group of tokens), and over how many warps the heads of a token are spread: so
+// many (of those that divide the warps of a CTA) that the last round of the groups over the warps costs least.
+void divide(RopeParams& p, int sms, int& ctas) {
+  const int lpr = p.d / 16, rows = 32 / lpr, pairs = p.rot / 2, warps = kThreads / 32;
+  auto steps = [&](int side, int hb) { return (p.heads[side] + hb - 1) / hb; };
+  double best = 0, fixed = 0;
+  for (int hb = 1; hb <= rows; ++hb) {
+    const double f = 60.0 + 40.0 * ((pairs + hb * lpr - 1) / (hb * lpr));
+    const double cost = (100.0 * (steps(0, hb) + steps(1, hb)) + (p.heads[1] ? 2 : 1) * f) / (rows / hb);
+    if (hb == 1 || cost < best) best = cost, fixed = f, p.hb = hb, p.tb = rows / hb;
+  }
+  const int64_t groups = (p.tokens + p.tb - 1) / p.tb, most = static_cast<int64_t>(kCtasPerSm) * sms;
+  for (int hs = 1; hs <= warps && hs < 2 * steps(0, p.hb); hs *= 2) {
+    double cost = 0;
+    for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
+      const double rounds = static_cast<double>(groups * hs) / (most * warps);
+      cost += (rounds < 1 ? 1 : rounds > 4 ? rounds : ceil(rounds)) * (fixed + 100.0 * ((steps(side, p.hb) + hs - 1) / hs));
+    }
+    if (hs == 1 || cost < best) best = cost, p.hs = hs;
+  }
+  const int64_t want = (groups * p.hs * (p.heads[1] ? 2 : 1) + warps - 1) / warps;
+  ctas = static_cast<int>(want < most ? want : most);
 }
 
 int elem_size(int dtype) { return dtype == WK_F32 ? 4 : 2; }
@@ -399,6 +654,7 @@ int fill(const wk_rope_args* a, bool bwd, RopeParams& p) {
   const bool keys = a->Hk > 0;
   if (keys && (!a->k || !a->k_out)) return WK_E_ARG;
   const bool norm = a->q_weight != nullptr;
+  if (norm && (!aligned16(a->q_weight) || (keys && !aligned16(a->k_weight)))) return WK_E_ARG;
   if (norm && (!known_dtype(a->w_dtype) || (keys && !a->k_weight) || !(a->eps >= 0.f))) return WK_E_ARG;
   if (bwd && (!norm || !a->dq_out || (keys && !a->dk_out) || !a->dq_weight || (keys && !a->dk_weight))) return WK_E_ARG;
   const bool fp8 = a->q_descale != nullptr;
@@ -434,10 +690,10 @@ int fill(const wk_rope_args* a, bool bwd, RopeParams& p) {
     p.ps[i] = a->position_strides[i];
   }
   for (int i = 0; i < 4; ++i) p.axis_map[i] = a->axis_map[i];
-  p.B = a->B, p.N = a->N, p.Hq = a->Hq, p.H = a->Hq + a->Hk;
+  p.N = a->N, p.heads[0] = a->Hq, p.heads[1] = a->Hk;
   p.tokens = static_cast<int>(tokens);
   p.d = a->d, p.rot = a->rot;
-  p.hkv = a->Hkv, p.group = fp8 ? a->Hq / a->Hkv : 1;
+  p.hkv = a->Hkv, p.inv_group = fp8 ? 1.f / static_cast<float>(a->Hq / a->Hkv) : 1.f;
   p.w_dtype = a->w_dtype, p.pos64 = a->position_int64, p.freq64 = a->inv_freq_f64;
   p.interleaved = a->interleaved != 0, p.inverse = a->inverse != 0;
   p.eps = a->eps;
@@ -445,27 +701,21 @@ int fill(const wk_rope_args* a, bool bwd, RopeParams& p) {
 }
 
 template <typename T, bool FP8, bool NORM>
-const void* forward_kernel(int lanes) {
-  switch (lanes) {
-    case 2: return reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 2>);
-    case 4: return reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 4>);
-    case 8: return reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 8>);
-    default: return reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 16>);
-  }
+const void* forward_kernel(int d) {
+  return d == 64    ? reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 4>)
+         : d == 128 ? reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 8>)
+                    : reinterpret_cast<const void*>(rope_kernel<T, FP8, NORM, 0>);
 }
 template <typename T>
-const void* forward_kernel(int lanes, bool fp8, bool norm) {
-  if (fp8) return norm ? forward_kernel<T, true, true>(lanes) : forward_kernel<T, true, false>(lanes);
-  return norm ? forward_kernel<T, false, true>(lanes) : forward_kernel<T, false, false>(lanes);
+const void* forward_kernel(int d, bool fp8, bool norm) {
+  if (fp8) return norm ? forward_kernel<T, true, true>(d) : forward_kernel<T, true, false>(d);
+  return norm ? forward_kernel<T, false, true>(d) : forward_kernel<T, false, false>(d);
 }
 template <typename T>
-const void* backward_kernel(int lanes) {
-  switch (lanes) {
-    case 2: return reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 2>);
-    case 4: return reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 4>);
-    case 8: return reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 8>);
-    default: return reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 16>);
-  }
+const void* backward_kernel(int d) {
+  return d == 64    ? reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 4>)
+         : d == 128 ? reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 8>)
+                    : reinterpret_cast<const void*>(norm_rope_bwd_kernel<T, 0>);
 }
 
 }  // namespace
@@ -478,22 +728,21 @@ extern "C" int wk_rope(const wk_rope_args* a, void* stream) {
   if (int unsupported = require_sm100()) return unsupported;
   const int sms = sm_count();
   if (sms <= 0) return WK_E_CUDA;
-  const int lanes = lanes_of(p.d);
   const bool fp8 = p.descale[0] != nullptr, norm = p.w[0] != nullptr;
-  p.per_cta = tokens_per_cta(p.tokens, p.H, p.d, sms);
-  const void* kernel = a->dtype == WK_BF16 ? forward_kernel<__nv_bfloat16>(lanes, fp8, norm)
-                       : a->dtype == WK_F16 ? forward_kernel<__half>(lanes, fp8, norm)
-                                            : forward_kernel<float>(lanes, fp8, norm);
-  const int smem = (p.per_cta * p.rot + (norm ? 2 * p.d : 0)) * 4;
-  const unsigned grid = static_cast<unsigned>((p.tokens + p.per_cta - 1) / p.per_cta);
-  return launch_pdl(kernel, dim3(grid), kThreads, smem, static_cast<cudaStream_t>(stream), 1, {&p});
+  int ctas;
+  divide(p, sms, ctas);
+  const void* kernel = a->dtype == WK_BF16 ? forward_kernel<__nv_bfloat16>(p.d, fp8, norm)
+                       : a->dtype == WK_F16 ? forward_kernel<__half>(p.d, fp8, norm)
+                                            : forward_kernel<float>(p.d, fp8, norm);
+  const int smem = kThreads / 32 * (a->dtype == WK_F32 ? kStages<float, false> * kRowBytes<float> : kStages<__half, false> * kRowBytes<__half>);
+  if (allow_smem(kernel, smem)) return WK_E_CUDA;
+  return launch_pdl(kernel, dim3(ctas), kThreads, smem, static_cast<cudaStream_t>(stream), 1, {&p});
 }
 
-extern "C" int64_t wk_qk_norm_rope_bwd_workspace_bytes(int B, int N, int heads, int d) {
+// Two rows of d sums per CTA.
+extern "C" int64_t wk_qk_norm_rope_bwd_workspace_bytes(int d) {
   const int sms = wk::sm_count();
-  if (B <= 0 || N <= 0 || heads <= 0 || d <= 0 || sms <= 0) return 0;
-  const int64_t tokens = static_cast<int64_t>(B) * N;
-  return static_cast<int64_t>(wk::bwd_ctas(tokens, wk::tokens_per_cta(tokens, heads, d, sms), sms)) * 2 * d * 4;
+  return d > 0 && sms > 0 ? static_cast<int64_t>(wk::kCtasPerSm) * sms * 2 * d * 4 : 0;
 }
 
 extern "C" int wk_qk_norm_rope_bwd(const wk_rope_args* a, void* stream) {
@@ -503,22 +752,20 @@ extern "C" int wk_qk_norm_rope_bwd(const wk_rope_args* a, void* stream) {
   if (int unsupported = require_sm100()) return unsupported;
   const int sms = sm_count();
   if (sms <= 0) return WK_E_CUDA;
-  if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15) ||
-      a->workspace_bytes < wk_qk_norm_rope_bwd_workspace_bytes(p.B, p.N, p.H, p.d))
-    return WK_E_ARG;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < wk_qk_norm_rope_bwd_workspace_bytes(p.d)) return WK_E_ARG;
   p.partial = static_cast<float*>(a->workspace);
-  const int lanes = lanes_of(p.d);
-  p.per_cta = tokens_per_cta(p.tokens, p.H, p.d, sms);
-  const int ctas = bwd_ctas(p.tokens, p.per_cta, sms);
-  const void* kernel = a->dtype == WK_BF16 ? backward_kernel<__nv_bfloat16>(lanes)
-                       : a->dtype == WK_F16 ? backward_kernel<__half>(lanes)
-                                            : backward_kernel<float>(lanes);
-  const int tables = (p.per_cta * p.rot + 2 * p.d) * 4, sums = kThreads / 32 * p.d * 4;
+  int ctas;
+  divide(p, sms, ctas);
+  const void* kernel = a->dtype == WK_BF16 ? backward_kernel<__nv_bfloat16>(p.d)
+                       : a->dtype == WK_F16 ? backward_kernel<__half>(p.d)
+                                            : backward_kernel<float>(p.d);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int bad = launch_pdl(kernel, dim3(ctas), kThreads, tables > sums ? tables : sums, st, 1, {&p})) return bad;
+  const int smem = kThreads / 32 * 2 * (a->dtype == WK_F32 ? kStages<float, true> * kRowBytes<float> : kStages<__half, true> * kRowBytes<__half>);
+  if (allow_smem(kernel, smem)) return WK_E_CUDA;
+  if (int bad = launch_pdl(kernel, dim3(ctas), kThreads, smem, st, 1, {&p})) return bad;
   const float* partial = p.partial;
-  int parts = ctas, d = p.d, w_dtype = p.w_dtype;
+  int d = p.d, w_dtype = p.w_dtype;
   void *dq = a->dq_weight, *dk = a->dk_weight;
-  return launch_pdl(reinterpret_cast<const void*>(dweight_kernel), dim3((d + 31) / 32, p.x[1] ? 2 : 1), 1024, 0, st, 1,
-                    {&partial, &parts, &d, &dq, &dk, &w_dtype});
+  return launch_pdl(reinterpret_cast<const void*>(dweight_kernel), dim3((d + 31) / 32, p.heads[1] ? 2 : 1), 1024, 0, st, 1,
+                    {&partial, &ctas, &d, &dq, &dk, &w_dtype});
 }

@@ -132,6 +132,12 @@ def _put(args, name, x):
     setattr(args, name + "_strides", (ctypes.c_int64 * 3)(*x.stride()[:3]))
 
 
+def _weight(w):
+    """``w`` where the kernels' 16-byte loads can read it."""
+    w = w.contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
 def _check_weights(q, k, q_weight, k_weight):
     d = q.shape[3]
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
@@ -201,8 +207,8 @@ def _forward(what, q, k, q_weight, k_weight, positions, inv_freq, eps, sections,
     if q.numel() == 0:
         return tuple(outs)
     if what == "qk_norm_rope":
-        q_weight = q_weight.contiguous()
-        k_weight = None if k is None else k_weight.contiguous()
+        q_weight = _weight(q_weight)
+        k_weight = None if k is None else _weight(k_weight)
         args.q_weight, args.w_dtype, args.eps = q_weight.data_ptr(), _DTYPES[q_weight.dtype], float(eps)
         args.k_weight = None if k is None else k_weight.data_ptr()
         keep += [q_weight, k_weight]
@@ -324,7 +330,7 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_fr
             dws.append(None)
             continue
         src, dsrc = (t if _direct(t, 16) else t.contiguous() for t in (x, dy))
-        w = w.contiguous()
+        w = _weight(w)
         grads.append(torch.empty_like(x))
         dws.append(torch.empty_like(w))
         _put(args, name, src)
@@ -338,7 +344,7 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_fr
     args.w_dtype, args.eps = _DTYPES[q_weight.dtype], float(eps)
     lib, host = _lib.lib(), _lib.host()
     with torch.cuda.device(q.device):
-        args.workspace_bytes = lib.wk_qk_norm_rope_bwd_workspace_bytes(args.B, args.N, args.Hq + args.Hk, args.d)
+        args.workspace_bytes = lib.wk_qk_norm_rope_bwd_workspace_bytes(args.d)
     workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=q.device)
     args.workspace = workspace.data_ptr()
     _lib.check(host.launch(_lib.address(lib.wk_qk_norm_rope_bwd), ctypes.addressof(args), q.device.index), "qk_norm_rope_bwd")
