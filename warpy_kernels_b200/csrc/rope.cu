@@ -34,9 +34,9 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kCtasPerSm = 3;
 constexpr int kMaxD = 256;
-// Rows of a warp that are under way: 16-bit types 6 KiB a warp and 96 KiB an SM forward, half again as many bytes otherwise.
+// Steps of a warp that are under way, two rows per lane each.
 template <typename T, bool BWD>
-constexpr int kStages = sizeof(T) == 2 ? (BWD ? 4 : 6) : (BWD ? 3 : 4);
+constexpr int kStages = sizeof(T) == 2 ? (BWD ? 3 : 4) : (BWD ? 2 : 3);
 constexpr int kTable = 512;  // cosines and sines of a warp's tokens: at most 32 rows / LPR . 8 LPR pairs
 
 struct RopeParams {
@@ -189,19 +189,24 @@ struct Place {
       at_a = 8 * in_row, at_b = at_a + p.rot / 2;
     }
   }
-  __device__ __forceinline__ float row_sum(float x) const {
+  // Two sums over the lanes of a row.
+  __device__ __forceinline__ void row_sums(float (&x)[2]) const {
     if (LPR) {
 #pragma unroll
-      for (int i = LPR / 2; i > 0; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-      return x;
+      for (int i = LPR / 2; i > 0; i >>= 1) {
+        const float a = __shfl_xor_sync(0xffffffffu, x[0], i), b = __shfl_xor_sync(0xffffffffu, x[1], i);
+        x[0] += a, x[1] += b;
+      }
+      return;
     }
     const int lane = threadIdx.x % 32;
 #pragma unroll
     for (int i = 8; i > 0; i >>= 1) {
-      const float y = __shfl_down_sync(0xffffffffu, x, i);
-      if (in_row < i && in_row + i < lpr) x += y;
+      const float a = __shfl_down_sync(0xffffffffu, x[0], i), b = __shfl_down_sync(0xffffffffu, x[1], i);
+      if (in_row < i && in_row + i < lpr) x[0] += a, x[1] += b;
     }
-    return __shfl_sync(0xffffffffu, x, lane - in_row);
+    x[0] = __shfl_sync(0xffffffffu, x[0], lane - in_row);
+    x[1] = __shfl_sync(0xffffffffu, x[1], lane - in_row);
   }
 };
 
@@ -366,24 +371,25 @@ struct Walk {
   }
 };
 
-// The rows that a lane fetches ahead into its ring: IN tensors (backward: also the gradients).
+// The rows that a lane fetches ahead into its ring: two heads at a step, `hb` apart, of IN tensors (backward: also the
+// gradients).
 template <typename T, int LPR, bool BWD>
 struct Fetcher {
-  static constexpr int IN = BWD ? 2 : 1, STAGES = kStages<T, BWD>, BYTES = IN * kRowBytes<T>;
+  static constexpr int IN = BWD ? 2 : 1, STAGES = kStages<T, BWD>, BYTES = 2 * IN * kRowBytes<T>;
   Walk<LPR> walk;
   uint32_t ring;
   int h, first, every, heads;
   const T* from[IN];
-  int64_t step[IN];
-  __device__ __forceinline__ Fetcher(const RopeParams& p, const Place<LPR>& at, uint32_t ring, int first, int every)
-      : walk(p, at), ring(ring), first(first), every(every) {
-    side(p, 0);
+  int64_t apart[IN];  // of the two heads
+  __device__ __forceinline__ Fetcher(const RopeParams& p, const Place<LPR>& at, uint32_t ring, int first)
+      : walk(p, at), ring(ring), first(first), every(2 * p.hs * p.hb) {
+    side(p);
     if (!walk.here()) go_on(p, at);
   }
-  __device__ __forceinline__ void side(const RopeParams& p, int which) {
-    heads = p.heads[which];
-    step[0] = every * p.xs[which][1];
-    if (BWD) step[IN - 1] = every * p.dys[which][1];
+  __device__ __forceinline__ void side(const RopeParams& p) {
+    heads = p.heads[walk.side];
+    apart[0] = p.hb * p.xs[walk.side][1];
+    if (BWD) apart[IN - 1] = p.hb * p.dys[walk.side][1];
     start(p);
   }
   __device__ __forceinline__ void start(const RopeParams& p) {
@@ -397,17 +403,19 @@ struct Fetcher {
   __device__ __forceinline__ void go_on(const RopeParams& p, const Place<LPR>& at) {
     if (walk.side || !p.heads[1]) return;
     walk.begin(p, at, 1);
-    side(p, 1);
+    side(p);
   }
   __device__ __forceinline__ void operator()(const RopeParams& p, const Place<LPR>& at, int stage) {
     if (walk.here()) {
-      if (at.active && walk.token < p.tokens && h < heads) {
+      const int there = at.active && walk.token < p.tokens ? heads - h : 0;
 #pragma unroll
-        for (int i = 0; i < IN; ++i) fetch_raw(ring + stage * BYTES + i * kRowBytes<T>, from[i], at.at_a, at.at_b);
+      for (int i = 0; i < IN; ++i) {
+        const uint32_t dst = ring + stage * BYTES + 2 * i * kRowBytes<T>;
+        if (there > 0) fetch_raw(dst, from[i], at.at_a, at.at_b);
+        if (there > p.hb) fetch_raw(dst + kRowBytes<T>, from[i] + apart[i], at.at_a, at.at_b);
+        from[i] += 2 * p.hs * apart[i];
       }
       h += every;
-#pragma unroll
-      for (int i = 0; i < IN; ++i) from[i] += step[i];
       if (h - at.hslot >= heads) {  // the same for the whole warp
         walk.next(p);
         if (walk.here()) start(p);
@@ -430,11 +438,11 @@ rope_kernel(const __grid_constant__ RopeParams p) {
   const uint32_t ring = smem_u32(ring_mem) + warp * Fetch::STAGES * Fetch::BYTES + (threadIdx.x % 32) * 16;
   const Place<LPR> at(p);
   const float inv_d = 1.f / static_cast<float>(p.d);
-  const int first = (blockIdx.x * WARPS + warp) % p.hs * p.hb + at.hslot, every = p.hs * p.hb;
+  const int first = (blockIdx.x * WARPS + warp) % p.hs * 2 * p.hb + at.hslot, every = 2 * p.hs * p.hb;
   pdl_launch_dependents();
   pdl_wait();
 
-  Fetch fetch(p, at, ring, first, every);
+  Fetch fetch(p, at, ring, first);
   for (int i = 0; i < Fetch::STAGES; ++i) fetch(p, at, i);
   int stage = 0;
   Walk<LPR> now(p, at);
@@ -448,40 +456,54 @@ rope_kernel(const __grid_constant__ RopeParams p) {
       weight8(p.w[side], p.w_dtype, at.at_a, w);
       weight8(p.w[side], p.w_dtype, at.at_b, w + 8);
     }
-    const int64_t to_step = every * p.ys[side][1];
+    const int64_t apart = p.hb * p.ys[side][1];
     for (; now.here(); now.next(p)) {
-      const bool live = at.active && now.token < p.tokens;
       uint64_t own[8], other[8];
+      const bool live = at.active && now.token < p.tokens;
       {
         float c[8], s[8];
         angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
         factors(c, s, w, at.turned, p.interleaved, own, other);
       }
       Out* to = static_cast<Out*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
-      for (int h = first; h - at.hslot < heads; h += every, to += to_step) {
-        const bool row = live && h < heads;
-        float scale = 1.f;
-        if (FP8 && row)  // h / group, exact: heads are fewer than 2^20
-          scale = p.descale[side][now.b * p.hkv + (side ? h : static_cast<int>((static_cast<float>(h) + 0.5f) * p.inv_group))];
-        asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
-        uint64_t v[8], y[8];
-        {
-          Raw<T> raw;
-          read_raw(ring + stage * Fetch::BYTES, raw);
-          unpack(raw, v);
-        }
-        float f = 1.f;
-        if (NORM) f = rsqrtf(at.row_sum(dot(v, v)) * inv_d + p.eps);
-        turn(v, own, other, at.turned, p.interleaved, y);
-        if (FP8) f *= __frcp_rn(scale);
-        if (NORM || FP8) {
-          const uint64_t f2 = pack_f32x2(f, f);
+      for (int h = first; h - at.hslot < heads; h += every, to += 2 * p.hs * apart) {
+        const int there = live ? heads - h : 0;
+        float scale[2] = {1.f, 1.f};
+        if (FP8) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = mul_f32x2(y[i], f2);
+          for (int i = 0; i < 2; ++i)
+            if (there > i * p.hb)  // head / group, exact: heads are fewer than 2^20
+              scale[i] = p.descale[side][now.b * p.hkv + static_cast<int>((static_cast<float>(h + i * p.hb) + 0.5f) *
+                                                                          (side ? 1.f : p.inv_group))];
         }
-        if (row) {
-          store8(to + at.at_a, y);
-          store8(to + at.at_b, y + 4);
+        asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
+        uint64_t v[2][8], y[8];
+        float f[2] = {1.f, 1.f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // where there is no second head, what lies there is read for nothing
+          Raw<T> raw;
+          read_raw(ring + stage * Fetch::BYTES + i * kRowBytes<T>, raw);
+          unpack(raw, v[i]);
+        }
+        if (NORM) {
+          float ss[2] = {dot(v[0], v[0]), dot(v[1], v[1])};
+          at.row_sums(ss);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) f[i] = rsqrtf(ss[i] * inv_d + p.eps);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          turn(v[i], own, other, at.turned, p.interleaved, y);
+          if (FP8) f[i] *= __frcp_rn(scale[i]);
+          if (NORM || FP8) {
+            const uint64_t f2 = pack_f32x2(f[i], f[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = mul_f32x2(y[j], f2);
+          }
+          if (there > i * p.hb) {
+            store8(to + i * apart + at.at_a, y);
+            store8(to + i * apart + at.at_b, y + 4);
+          }
         }
         fetch(p, at, stage);  // into the place that has just been read
         if (++stage == Fetch::STAGES) stage = 0;
@@ -502,11 +524,11 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
   const uint32_t ring = smem_u32(ring_mem) + warp * Fetch::STAGES * Fetch::BYTES + (threadIdx.x % 32) * 16;
   const Place<LPR> at(p);
   const float inv_d = 1.f / static_cast<float>(p.d);
-  const int first = (blockIdx.x * WARPS + warp) % p.hs * p.hb + at.hslot, every = p.hs * p.hb;
+  const int first = (blockIdx.x * WARPS + warp) % p.hs * 2 * p.hb + at.hslot, every = 2 * p.hs * p.hb;
   pdl_launch_dependents();
   pdl_wait();
 
-  Fetch fetch(p, at, ring, first, every);
+  Fetch fetch(p, at, ring, first);
   for (int i = 0; i < Fetch::STAGES; ++i) fetch(p, at, i);
   int stage = 0;
   Walk<LPR> now(p, at);
@@ -523,37 +545,42 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = pack_f32x2(v[2 * i], v[2 * i + 1]), dw[i] = 0;
     }
-    const int64_t to_step = every * p.ys[side][1];
+    const int64_t apart = p.hb * p.ys[side][1];
     for (; now.here(); now.next(p)) {
       const bool live = at.active && now.token < p.tokens;
       float c[8], s[8];
       angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
       T* to = static_cast<T*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
-      for (int head = first; head - at.hslot < heads; head += every, to += to_step) {
+      for (int head = first; head - at.hslot < heads; head += every, to += 2 * p.hs * apart) {
+        const int there = live ? heads - head : 0;
         asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
-        uint64_t x[8], g[8], h[8];
-        {
-          Raw<T> raw;
-          uint64_t dy[8];
-          read_raw(ring + stage * Fetch::BYTES + kRowBytes<T>, raw);
-          unpack(raw, dy);
-          turn_back(dy, c, s, at.turned, p.interleaved, g);
-          read_raw(ring + stage * Fetch::BYTES, raw);
-          unpack(raw, x);
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = mul_f32x2(g[i], w[i]);
-        const float ss = at.row_sum(dot(x, x)), hx = at.row_sum(dot(h, x));
-        const float f = rsqrtf(ss * inv_d + p.eps), m = -f * f * f * hx * inv_d;
-        const uint64_t f2 = pack_f32x2(f, f), m2 = pack_f32x2(m, m);
-        if (live && head < heads) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            dw[i] = fma_f32x2(mul_f32x2(g[i], x[i]), f2, dw[i]);
-            h[i] = fma_f32x2(x[i], m2, mul_f32x2(h[i], f2));
+        for (int i = 0; i < 2; ++i) {
+          uint64_t x[8], g[8], h[8];
+          {
+            Raw<T> raw;
+            uint64_t dy[8];
+            read_raw(ring + stage * Fetch::BYTES + (2 + i) * kRowBytes<T>, raw);
+            unpack(raw, dy);
+            turn_back(dy, c, s, at.turned, p.interleaved, g);
+            read_raw(ring + stage * Fetch::BYTES + i * kRowBytes<T>, raw);
+            unpack(raw, x);
           }
-          store8(to + at.at_a, h);
-          store8(to + at.at_b, h + 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = mul_f32x2(g[j], w[j]);
+          float sum[2] = {dot(x, x), dot(h, x)};
+          at.row_sums(sum);
+          const float f = rsqrtf(sum[0] * inv_d + p.eps), m = -f * f * f * sum[1] * inv_d;
+          const uint64_t f2 = pack_f32x2(f, f), m2 = pack_f32x2(m, m);
+          if (there > i * p.hb) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              dw[j] = fma_f32x2(mul_f32x2(g[j], x[j]), f2, dw[j]);
+              h[j] = fma_f32x2(x[j], m2, mul_f32x2(h[j], f2));
+            }
+            store8(to + i * apart + at.at_a, h);
+            store8(to + i * apart + at.at_b, h + 4);
+          }
         }
         fetch(p, at, stage);
         if (++stage == Fetch::STAGES) stage = 0;
@@ -617,30 +644,39 @@ dweight_kernel(const float* __restrict__ partial, int parts, int d, void* dw_q, 
     static_cast<__half*>(out)[col] = __float2half_rn(s);
 }
 
-// How a warp's rows are divided into heads and tokens: the division that takes the fewest instructions per token (100 for a
-// step over its rows, 40 for an angle, 60 for a group of tokens), and over how many warps the heads of a token are spread: so
-// many (of those that divide the warps of a CTA) that the last round of the groups over the warps costs least.
-void divide(RopeParams& p, int sms, int& ctas) {
-  const int lpr = p.d / 16, rows = 32 / lpr, pairs = p.rot / 2, warps = kThreads / 32;
-  auto steps = [&](int side, int hb) { return (p.heads[side] + hb - 1) / hb; };
+// How a warp's rows are divided into heads and tokens: the division that takes the fewest instructions per token (150 for a
+// step over two rows per lane, 40 for an angle, 60 for a group of tokens), and over how many warps the heads of a token are
+// spread: so many (of those that divide the warps of a CTA) that the last round of the groups over the warps costs least.
+void divide(RopeParams& p, int ctas_at_once, int& ctas) {
+  const int lpr = p.d / 16, rows = 32 / lpr, pairs = p.rot / 2, warps = kThreads / 32, sides = p.heads[1] ? 2 : 1;
+  auto steps = [&](int side, int hb) { return (p.heads[side] + 2 * hb - 1) / (2 * hb); };
   double best = 0, fixed = 0;
   for (int hb = 1; hb <= rows; ++hb) {
     const double f = 60.0 + 40.0 * ((pairs + hb * lpr - 1) / (hb * lpr));
-    const double cost = (100.0 * (steps(0, hb) + steps(1, hb)) + (p.heads[1] ? 2 : 1) * f) / (rows / hb);
+    const double cost = (150.0 * (steps(0, hb) + steps(1, hb)) + sides * f) / (rows / hb);
     if (hb == 1 || cost < best) best = cost, fixed = f, p.hb = hb, p.tb = rows / hb;
   }
-  const int64_t groups = (p.tokens + p.tb - 1) / p.tb, most = static_cast<int64_t>(kCtasPerSm) * sms;
+  const int64_t groups = (p.tokens + p.tb - 1) / p.tb;
   for (int hs = 1; hs <= warps && hs < 2 * steps(0, p.hb); hs *= 2) {
     double cost = 0;
-    for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
-      const double rounds = static_cast<double>(groups * hs) / (most * warps);
-      cost += (rounds < 1 ? 1 : rounds > 4 ? rounds : ceil(rounds)) * (fixed + 100.0 * ((steps(side, p.hb) + hs - 1) / hs));
+    for (int side = 0; side < sides; ++side) {
+      const double rounds = static_cast<double>(groups * hs) / (static_cast<double>(ctas_at_once) * warps);
+      cost += (rounds < 1 ? 1 : rounds > 4 ? rounds : ceil(rounds)) * (fixed + 150.0 * ((steps(side, p.hb) + hs - 1) / hs));
     }
     if (hs == 1 || cost < best) best = cost, p.hs = hs;
   }
-  const int64_t want = (groups * p.hs * (p.heads[1] ? 2 : 1) + warps - 1) / warps;
-  ctas = static_cast<int>(want < most ? want : most);
+  const int64_t want = (groups * p.hs * sides + warps - 1) / warps;
+  ctas = static_cast<int>(want < ctas_at_once ? want : ctas_at_once);
 }
+
+// CTAs that fit the GPU by their shared memory (`fixed`: the static part).
+int ctas_at_once(int sms, int smem, int fixed) {
+  const int fit = 227 * 1024 / (smem + fixed + 1024);
+  return sms * (fit < kCtasPerSm ? fit : kCtasPerSm);
+}
+template <typename T, bool BWD>
+constexpr int kRingBytes = kThreads / 32 * Fetcher<T, 0, BWD>::STAGES * Fetcher<T, 0, BWD>::BYTES;
+constexpr int kTableBytes = kThreads / 32 * kTable * 4, kSumBytes = 2 * kThreads / 32 * kMaxD * 4;
 
 int elem_size(int dtype) { return dtype == WK_F32 ? 4 : 2; }
 bool known_dtype(int t) { return t == WK_BF16 || t == WK_F32 || t == WK_F16; }
@@ -729,12 +765,12 @@ extern "C" int wk_rope(const wk_rope_args* a, void* stream) {
   const int sms = sm_count();
   if (sms <= 0) return WK_E_CUDA;
   const bool fp8 = p.descale[0] != nullptr, norm = p.w[0] != nullptr;
-  int ctas;
-  divide(p, sms, ctas);
   const void* kernel = a->dtype == WK_BF16 ? forward_kernel<__nv_bfloat16>(p.d, fp8, norm)
                        : a->dtype == WK_F16 ? forward_kernel<__half>(p.d, fp8, norm)
                                             : forward_kernel<float>(p.d, fp8, norm);
-  const int smem = kThreads / 32 * (a->dtype == WK_F32 ? kStages<float, false> * kRowBytes<float> : kStages<__half, false> * kRowBytes<__half>);
+  const int smem = a->dtype == WK_F32 ? kRingBytes<float, false> : kRingBytes<__half, false>;
+  int ctas;
+  divide(p, ctas_at_once(sms, smem, kTableBytes), ctas);
   if (allow_smem(kernel, smem)) return WK_E_CUDA;
   return launch_pdl(kernel, dim3(ctas), kThreads, smem, static_cast<cudaStream_t>(stream), 1, {&p});
 }
@@ -754,14 +790,14 @@ extern "C" int wk_qk_norm_rope_bwd(const wk_rope_args* a, void* stream) {
   if (sms <= 0) return WK_E_CUDA;
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < wk_qk_norm_rope_bwd_workspace_bytes(p.d)) return WK_E_ARG;
   p.partial = static_cast<float*>(a->workspace);
-  int ctas;
-  divide(p, sms, ctas);
   const void* kernel = a->dtype == WK_BF16 ? backward_kernel<__nv_bfloat16>(p.d)
                        : a->dtype == WK_F16 ? backward_kernel<__half>(p.d)
                                             : backward_kernel<float>(p.d);
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int smem = kThreads / 32 * 2 * (a->dtype == WK_F32 ? kStages<float, true> * kRowBytes<float> : kStages<__half, true> * kRowBytes<__half>);
+  const int smem = a->dtype == WK_F32 ? kRingBytes<float, true> : kRingBytes<__half, true>;
+  int ctas;
+  divide(p, ctas_at_once(sms, smem, kTableBytes + kSumBytes), ctas);
   if (allow_smem(kernel, smem)) return WK_E_CUDA;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int bad = launch_pdl(kernel, dim3(ctas), kThreads, smem, st, 1, {&p})) return bad;
   const float* partial = p.partial;
   int d = p.d, w_dtype = p.w_dtype;
