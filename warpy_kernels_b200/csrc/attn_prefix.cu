@@ -5,28 +5,30 @@
 //
 // Attending sequence by sequence reads the prefix once per sequence.  Here the query rows of ALL sequences that share a KV
 // head are stacked, 128 to a tile, and go over the prefix together; the rows of one sequence (its group of query heads
-// times its queries) go over its own keys.  Both are the same work: a unit is up to 128 rows and a range of 64-key tiles,
-// S = Q.K^T and O += P.V with 128 x 64 tiles on tcgen05.  A sequence's few rows leave most of a tile empty, which costs
-// nothing: those units wait for memory (a tile of 128 x 64 takes the tensor pipe 512 cycles, its keys 700 at an SM's share
-// of the memory bandwidth), and the warps of empty rows skip the softmax.
+// times its queries) go over its own keys.
 //
-// Work division: all tiles of all units form one line, prefix first, that is cut into as many equal pieces as CTAs fit the
-// GPU (a tile of own keys counts more than one of the prefix).  Lengths are read on the device.  A CTA's piece of a unit is
-// a segment; every segment leaves a partial result (O / l and the log-sum-exp of its rows, fp32) and a second kernel, set up
-// beside the first, adds up the segments of every row, in the order of the line.
+// Own keys come first, and leave parts: O / l and the log-sum-exp of every row, fp32.  Up to 32 rows a sequence, that is a
+// kernel on mma.sync whose warps work by themselves (bound by memory, and by latency where sequences are short); more
+// rows take the tensor-core kernel below, one CTA for 128 of them.
+// The prefix: a unit is 128 stacked rows, and S = Q.K^T and O += P.V go by 128 x 64 tiles on tcgen05.  A unit's tiles are
+// divided over the CTAs of a cluster, which meet in distributed shared memory, add the own keys' parts and write the output.
+// Where units are few, several clusters share one; then they leave parts too, and a last kernel adds up all of them.  The
+// prefix kernel is set up and runs beside the one for own keys and waits for its end before it reads its parts.
 //
-// One CTA (two per SM, 320 threads): warp 0 TMA producer, warp 1 issues the products, two softmax groups of four warps take
-// the tiles in turn, one thread per row: the structure of attn_fwd_bf16.cu, persistent over its segments.  P is bf16 and
+// One CTA of the tensor-core kernel (two per SM, 320 threads): warp 0 TMA producer, warp 1 issues the products, two softmax
+// groups of four warps take the tiles in turn, one thread per row: the structure of attn_fwd_bf16.cu.  P is bf16 and
 // overwrites its scores in tensor memory.  FP8: scores from e4m3 (kind::f8f6f4); V tiles are converted to bf16 (exact) in
 // shared memory by the group that has the tile, so that P keeps 8 bits.
 //
-// Numerics: logits in base 2; the row reference is the maximum of the segment's first tile (bf16 has the exponent range to
-// leave it there).  A segment in which a row rises more than 2^60 above its reference is gone through again at the end of
-// its CTA, with the maxima it then knows.
+// Numerics: logits in base 2.  Tensor-core kernel: the row reference is the maximum of the CTA's first tile (bf16 has the
+// exponent range to leave it there); a CTA in which a row rises more than 2^60 above it goes through its keys once more, with
+// the maxima it then knows.  Kernel for few rows: the moving reference of attn_rows.cu.
 #include <math.h>
 
 #include "common.cuh"
 #include "host_common.h"
+#include "pair.cuh"
+#include "rows16.cuh"
 #include "softmax16.cuh"
 
 namespace wk {
@@ -40,11 +42,17 @@ constexpr int X_TMEM_COLS = 256;
 constexpr int X_S_COLS = 64;  // buffer b at column 64 b; P over its first 32
 constexpr int X_O_COL = 128;
 constexpr float X_MAX_EXP = 60.f;
-constexpr int X_CUM = 1024;   // sequences whose tile counts are kept in shared memory
-constexpr int X_FLAGS = 512;  // segments of a CTA that are told apart when they are gone through again
+constexpr int X_CLUSTER = 16;  // largest cluster
+constexpr int X_PAD = 4;       // values between rows in the exchange: lanes with neighbouring rows write without conflicts
+
+constexpr int Y_STAGES = 3;
+constexpr int Y_START = 1;  // what a unit of the kernel for few rows weighs beside its steps
+constexpr int Y_WARPS = R_WARPS;
+constexpr int Y_FEW_ROWS = 32;  // rows of a sequence up to which that kernel takes them
+constexpr int Y_CUM = 1024;     // sequences whose weights are summed in shared memory
 
 struct PrefixParams {
-  const uint8_t* q;
+  const uint8_t *q, *k, *v;  // k, v: own keys and values
   const float* q_descale;
   const float* kp_descale;
   const float* vp_descale;
@@ -53,145 +61,84 @@ struct PrefixParams {
   const int* seqused;
   __nv_bfloat16* out;
   float* lse;
-  int64_t q_strides[3];  // bytes
-  int64_t out_strides[3], lse_strides[2];
+  int64_t q_strides[3], k_strides[3], v_strides[3];  // bytes
+  int64_t out_strides[3], lse_strides[2];            // elements
   int B, Hq, Hkv, group, Nq, P, S;
-  int rows_all;      // stacked rows of a KV head: B . group . Nq
-  int rows_own;      // of one sequence
-  int own_slot;      // rows that a partial result of own keys has room for: min(128, rows_own)
-  int units_p;       // Hkv . ceil(rows_all / 128), 0 without a prefix
-  int blocks_p;      // ceil(rows_all / 128)
-  int blocks_own;    // ceil(rows_own / 128)
-  int tiles_p;       // of the prefix
-  int ctas;          // grid of the main kernel
-  int weight_p, weight_own;
+  int rows_all;    // stacked rows of a KV head: B . group . Nq
+  int rows_own;    // of one sequence
+  int blocks_p;    // units of a KV head's stacked rows
+  int tiles_p;     // of the prefix
+  int cluster;     // CTAs of a cluster
+  int splits;      // clusters that share a unit
+  int by_rows;     // own keys go to the kernel for few rows
+  int blocks_own;  // units of a sequence's rows: 16 rows each, or 128
+  int own_slot;    // rows of one of their parts
+  int pieces;      // by_rows: pieces that the line of units may be cut into
   int causal, lse_natural;
   float scale_log2;  // softmax_scale . log2(e)
-  int* cum;          // [B + 1] tiles of own keys before each sequence
-  float* part;       // [row slot][DH]
+  int* cum;          // [B + 1] by_rows: weight of the sequences' units before each of them
+  float* part;       // O / l of row slots [DH]: the prefix's, 128 a unit and split, then those of own keys
   float* part_lse;   // [row slot]
-  float* part_top;   // [row slot] largest score
+  int64_t own_parts;  // first row slot of own keys
   int* status;
 };
 
-// The line of tiles and its division.
-struct Line {
-  int Wp, W;   // weight of the prefix, of everything
-  int G;       // pieces
-  int wp, ws;  // weight of a tile
-};
-__device__ __forceinline__ Line make_line(const PrefixParams& p, int own_tiles) {
-  Line l;
-  const int per_seq = p.Hkv * p.blocks_own;
-  const int tp = p.units_p * p.tiles_p, ts = own_tiles * per_seq;
-  const bool few = tp + ts <= 4 * p.ctas;  // then the tiles are dealt out as evenly as they are
-  l.wp = few ? 1 : p.weight_p, l.ws = few ? 1 : p.weight_own;
-  l.Wp = tp * l.wp;
-  l.W = l.Wp + ts * l.ws;
-  l.G = min(p.ctas, l.W / max(l.wp, l.ws));  // every piece is at least one tile long
-  return l;
-}
-__device__ __forceinline__ int piece_start(const Line& l, int c) {
-  return static_cast<int>(static_cast<int64_t>(l.W) * c / l.G);
-}
-// The piece that weight x lies in.
-__device__ __forceinline__ int owner(const Line& l, int x) {
-  return static_cast<int>((static_cast<int64_t>(x + 1) * l.G - 1) / l.W);
+// Own keys of sequence b.
+__device__ __forceinline__ int own_keys(const PrefixParams& p, int b) {
+  return p.seqused ? max(0, min(p.S, __ldcg(p.seqused + b))) : p.S;
 }
 
-struct Segment {
-  bool own;
-  int b, h;        // sequence (own keys) and KV head
-  int row0, rows;  // of the unit's row space: stacked rows of the head, or rows of the sequence
-  int tile0, tiles;
-  int keys;        // length of the key range that tiles count in
-  int64_t slot;    // first row slot
-};
-
-// The segments of piece c, one after the other.
-struct Walker {
-  const PrefixParams& p;
-  const Line& l;
-  const int* cum;
-  int c, x, x1, b;
-  __device__ __forceinline__ Walker(const PrefixParams& p, const Line& l, const int* cum, int c)
-      : p(p), l(l), cum(cum), c(c), x(0), x1(0), b(-1) {
-    if (c < l.G) x = piece_start(l, c), x1 = piece_start(l, c + 1);
+// A line of W units of weight, cut into G pieces whose lengths differ by one at most.
+struct Pieces {
+  int W, G;
+  int size, longer;  // of a piece; how many (the first ones) are one longer
+  __device__ __forceinline__ Pieces(int weight, int most) {
+    W = weight, G = min(weight, most);
+    size = G ? W / G : 0;
+    longer = W - size * G;
   }
-  __device__ __forceinline__ bool next(Segment& s) {
-    while (x < x1) {
-      int base, w, total;
-      if (x < l.Wp) {
-        w = l.wp, total = p.tiles_p;
-        const int u = x / (total * w);
-        base = u * total * w;
-        s.own = false;
-        s.h = u / p.blocks_p, s.b = 0;
-        s.row0 = (u - s.h * p.blocks_p) * X_ROWS;
-        s.rows = min(X_ROWS, p.rows_all - s.row0);
-        s.keys = p.P;
-        s.slot = static_cast<int64_t>(u + c) * X_ROWS;
-      } else {
-        w = l.ws;
-        const int per_seq = p.Hkv * p.blocks_own;
-        const int y = (x - l.Wp) / w;  // a tile (x need not be at its start: rounding down stays in it)
-        if (b < 0) {  // the last sequence that starts at or before y
-          int lo = 0, hi = p.B - 1;
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (cum[mid] * per_seq <= y) lo = mid; else hi = mid - 1;
-          }
-          b = lo;
-        }
-        while (cum[b + 1] * per_seq <= y) ++b;
-        const int first = cum[b] * per_seq;
-        total = cum[b + 1] - cum[b];
-        const int u = (y - first) / total;
-        base = l.Wp + (first + u * total) * w;
-        s.own = true;
-        s.b = b, s.h = u / p.blocks_own;
-        s.row0 = (u - s.h * p.blocks_own) * X_ROWS;
-        s.rows = min(X_ROWS, p.rows_own - s.row0);
-        s.keys = p.seqused ? max(0, min(p.S, p.seqused[b])) : p.S;
-        s.slot = static_cast<int64_t>(p.units_p + p.ctas) * X_ROWS + static_cast<int64_t>(b * per_seq + u + c) * p.own_slot;
-      }
-      s.tile0 = (x - base + w - 1) / w;
-      const int end = min(total, (x1 - base + w - 1) / w);
-      s.tiles = end - s.tile0;
-      x = end == total ? base + total * w : x1;
-      if (s.tiles > 0) return true;
+  __device__ __forceinline__ int start(int c) const { return c * size + min(c, longer); }
+  // The piece that weight x lies in.
+  __device__ __forceinline__ int owner(int x) const {
+    const int edge = longer * (size + 1);
+    return x < edge ? x / (size + 1) : longer + (x - edge) / size;
+  }
+};
+// First row slot of the part that a piece leaves of a unit of own keys.
+__device__ __forceinline__ int64_t own_slot_of(const PrefixParams& p, int unit, int piece) {
+  return p.own_parts + static_cast<int64_t>(unit + piece) * p.own_slot;
+}
+
+// The parts that own keys have left of a row (row `own` of sequence b at KV head h): their row slots are
+// first + i . distance.
+struct OwnParts {
+  int64_t first;
+  int count, distance;
+  __device__ __forceinline__ OwnParts(const PrefixParams& p, int b, int h, int own) : first(0), count(0), distance(p.own_slot) {
+    if (!p.S) return;
+    if (p.by_rows) {
+      const int all = __ldcg(p.cum + p.B), before = __ldcg(p.cum + b), weight = __ldcg(p.cum + b + 1) - before;
+      if (weight <= Y_START) return;
+      const int per_seq = p.Hkv * p.blocks_own, u = h * p.blocks_own + own / R_ROWS, x = before * per_seq + u * weight;
+      const Pieces line(all * per_seq, p.pieces);
+      const int c = line.owner(x + Y_START);
+      count = line.owner(x + weight - 1) - c + 1;
+      first = own_slot_of(p, b * per_seq + u, c) + own % R_ROWS;
+    } else if (own_keys(p, b)) {
+      count = 1;
+      first = own_slot_of(p, (b * p.Hkv + h) * p.blocks_own + own / X_ROWS, 0) + own % X_ROWS;
     }
-    return false;
   }
 };
 
-// Exclusive sums of the sequences' tile counts, by the whole CTA; `cum` is in shared or global memory.
-__device__ __forceinline__ void sum_tiles(const PrefixParams& p, int* cum, int* warp_sums) {
-  const int per = (p.B + X_THREADS - 1) / X_THREADS, b0 = threadIdx.x * per, b1 = min(p.B, b0 + per);
-  auto tiles = [&](int b) {
-    const int n = p.seqused ? max(0, min(p.S, p.seqused[b])) : p.S;
-    return (n + X_KEYS - 1) / X_KEYS;
-  };
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += tiles(b);
-  int scan = sum;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-#pragma unroll
-  for (int i = 1; i < 32; i *= 2) {
-    const int other = __shfl_up_sync(0xffffffffu, scan, i);
-    if (lane >= i) scan += other;
-  }
-  if (lane == 31) warp_sums[warp] = scan;
-  __syncthreads();
-  int at = scan - sum;
-  for (int w = 0; w < warp; ++w) at += warp_sums[w];
-  for (int b = b0; b < b1; ++b) {
-    cum[b] = at;
-    at += tiles(b);
-  }
-  if (b1 == p.B && b0 < p.B) cum[p.B] = at;
-  __syncthreads();
-}
+// How a row of the tensor-core kernel ends.
+struct RowEnd {
+  float weight[X_CLUSTER];  // of the members' parts
+  float top, inv;           // reference of all weights, 1 / their sum
+  int64_t first;            // own keys' parts, to be weighted with 2^(lse - top)
+  int64_t to;               // offset in the output, or row slot
+  int parts;
+};
 
 template <bool FP8, int DH>
 struct PrefixCfg {
@@ -208,17 +155,16 @@ struct PrefixCfg {
   static constexpr int K_AT = Q_BYTES;
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
   static constexpr int V16_AT = V_AT + STAGES * K_BYTES;  // FP8 only: two buffers
+  // row reference, then l and largest score of each group; at the end the log-sum-exp of each row
   static constexpr int X_AT = V16_AT + (FP8 ? 2 * V16_BYTES : 0);
-  // exchange: row reference, then l and largest score of each group; segments to go through again; warp sums
-  static constexpr int FLAG_AT = X_AT + 5 * X_ROWS * 4;
-  static constexpr int CUM_AT = FLAG_AT + X_FLAGS / 8 + 64;
-  static constexpr int BAR_AT = CUM_AT + (X_CUM + 4) * 4;
+  static constexpr int ROW_AT = X_AT + 5 * X_ROWS * 4;  // where each row of Q is
+  static constexpr int BAR_AT = ROW_AT + X_ROWS * 8;
   static constexpr int SMEM = BAR_AT + 8 * (4 * STAGES + 8) + 16 + 1024;
+  // the exchange of a cluster takes the place of the tiles
+  static constexpr int PART_BYTES = X_ROWS * (DH + X_PAD) * 4;
+  static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowEnd)) <= X_AT, "");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -244,16 +190,16 @@ __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_
   lo = x[0], hi = x[1];
 }
 
-template <bool FP8, int DH>
+// OWN: the rows of one sequence over its own keys, one CTA for 128 rows, which leaves a part.  Else: stacked rows over the
+// prefix.
+template <bool FP8, int DH, bool OWN>
 __global__ void __launch_bounds__(X_THREADS, 2)
-attn_prefix_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_constant__ CUtensorMap map_vp,
-                   const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ PrefixParams p) {
   using C = PrefixCfg<FP8, DH>;
   constexpr int ST = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem_ptr = smem_raw + (smem - smem_u32(smem_raw));
   const uint32_t bars = smem + C::BAR_AT;
   auto k_full = [&](int s) { return bars + 8u * s; };
   auto k_empty = [&](int s) { return bars + 8u * (ST + s); };
@@ -262,9 +208,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
   const uint32_t misc = bars + 8u * 4 * ST;
   auto s_full = [&](int b) { return misc + 8u * b; };
   auto p_full = [&](int b) { return misc + 8u * (2 + b); };
-  const uint32_t q_full = misc + 8u * 4, o_full = misc + 8u * 5, o_free = misc + 8u * 6, tmem_slot = misc + 8u * 7;
-  volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem_ptr + C::FLAG_AT);
-  int* warp_sums = reinterpret_cast<int*>(smem_ptr + C::FLAG_AT + X_FLAGS / 8);
+  const uint32_t q_full = misc + 8u * 4, o_full = misc + 8u * 5, tmem_slot = misc + 8u * 6;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -280,437 +224,723 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_kp, const __grid_cons
     }
     mbar_init(q_full, X_SOFTMAX);
     mbar_init(o_full, 1);
-    mbar_init(o_free, X_SOFTMAX);
     mbar_fence_init();
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
   }
-  if (threadIdx.x < X_FLAGS / 32) flags[threadIdx.x] = 0;
   if (warp == 1) {
     tmem_alloc(tmem_slot, X_TMEM_COLS);
     tmem_relinquish();
+  }
+  // the unit: sequence (own keys), KV head, first row, rows, this CTA's tiles
+  int b = 0, h, row0, rows, tile0, tiles, keys;
+  if (OWN) {
+    const int u = blockIdx.x / p.blocks_own;
+    row0 = (blockIdx.x - u * p.blocks_own) * X_ROWS;
+    b = u / p.Hkv, h = u - b * p.Hkv;
+    rows = min(X_ROWS, p.rows_own - row0);
+  } else {
+    const int share = blockIdx.x % (p.cluster * p.splits), u = blockIdx.x / (p.cluster * p.splits);
+    h = u / p.blocks_p, row0 = (u - h * p.blocks_p) * X_ROWS;
+    rows = min(X_ROWS, p.rows_all - row0);
+    keys = p.P;
+    const int shares = p.cluster * p.splits, each = p.tiles_p / shares, more = p.tiles_p - each * shares;
+    tile0 = share * each + min(share, more);
+    tiles = each + (share < more);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  // Beside the kernel for own keys, what kernels before that one wrote is read through L2 only, by TMA behind a proxy fence.
+  const bool beside = !OWN && p.S > 0;
+  if (!beside) pdl_wait();
   pdl_launch_dependents();
-  pdl_wait();
-  // every CTA writes the same counts where they do not fit shared memory; the combining kernel reads them from there
-  int* cum = p.B <= X_CUM ? reinterpret_cast<int*>(smem_ptr + C::CUM_AT) : p.cum;
-  sum_tiles(p, cum, warp_sums);
-  if (blockIdx.x == 0 && cum != p.cum)
-    for (int i = threadIdx.x; i <= p.B; i += X_THREADS) p.cum[i] = cum[i];
-  const Line line = make_line(p, cum[p.B]);
+  if (OWN) {
+    keys = own_keys(p, b);
+    tile0 = 0, tiles = (keys + X_KEYS - 1) / X_KEYS;
+  }
 
-  int J = 0;       // tiles of the segments before this one
-  int n_seg = 0;   // segments before this one, over both passes
   bool ok = true;  // no wait of this thread's role has given up
-  for (int pass = 0; pass < 2; ++pass) {
-    Walker walk(p, line, cum, blockIdx.x);
-    Segment s;
-    for (int i = 0; walk.next(s); ++i) {
-      const int flag = min(i, X_FLAGS - 1);
-      if (pass && !(flags[flag / 32] >> (flag % 32) & 1)) continue;
-      if (warp == 0) {
-        if (lane == 0) {
-          const CUtensorMap* mk = s.own ? &map_k : &map_kp;
-          const CUtensorMap* mv = s.own ? &map_v : &map_vp;
-          for (int j = 0; ok && j < s.tiles; ++j) {
-            const int st = (J + j) % ST;
-            const uint32_t ph = ((J + j) / ST) & 1;
-            const int key0 = (s.tile0 + j) * X_KEYS;
-            ok = mbar_wait(k_empty(st), ph ^ 1, p.status, WK_ERR_TIMEOUT_EMPTY);
-            if (!ok) break;
-            mbar_expect_tx(k_full(st), C::K_BYTES);
-            for (int c = 0; c < C::SPANS; ++c)
-              tma_load_4d(smem + C::K_AT + st * C::K_BYTES + c * C::KV_SPAN, mk, k_full(st), 64 * c, key0, s.h, s.b);
-            ok = mbar_wait(v_empty(st), ph ^ 1, p.status, WK_ERR_TIMEOUT_EMPTY);
-            if (!ok) break;
-            mbar_expect_tx(v_full(st), C::K_BYTES);
-            for (int c = 0; c < C::SPANS; ++c)
-              tma_load_4d(smem + C::V_AT + st * C::K_BYTES + c * C::KV_SPAN, mv, v_full(st), 64 * c, key0, s.h, s.b);
-          }
-        }
-        __syncwarp();
-      } else if (warp == 1) {
-        const bool mine = elect_one();
-        constexpr uint32_t idesc_qk = FP8 ? make_idesc(0, 0, 0, 0, X_ROWS, X_KEYS) : make_idesc(1, 1, 0, 0, X_ROWS, X_KEYS);
-        constexpr uint32_t idesc_pv = make_idesc(1, 1, 0, 1, X_ROWS, DH);
-        const uint64_t q_desc = smem_desc_sw128(smem + C::Q_AT, 16, 1024);
-        ok = ok && mbar_wait_warp(q_full, n_seg & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-        // the tensor pipe runs in issue order: the scores also wait for the product that last read their buffer
-        auto issue_qk = [&](int j) {
+  float lse_row = -INFINITY, inv_row = 0.f;  // softmax threads: of their row, what its O is multiplied with
+  float m_ref = -INFINITY;
+  for (int pass = 0; tiles > 0; ++pass) {
+    const int J = pass * tiles;  // tiles before this pass
+    bool far = false;
+    if (warp == 0) {
+      if (lane == 0) {
+        if (beside) pdl_acquire_async();
+        for (int j = 0; ok && j < tiles; ++j) {
           const int st = (J + j) % ST;
-          ok = ok && mbar_wait_warp(k_full(st), ((J + j) / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-          if (!ok) return;
-          tc_fence_after();
-          const uint64_t k_desc = smem_desc_sw128(smem + C::K_AT + st * C::K_BYTES, 16, 1024);
-          const uint32_t d = tmem + ((J + j) & 1) * X_S_COLS;
-          if (mine) {
-#pragma unroll
-            for (int k = 0; k < DH * C::SIZE / 32; ++k) {  // 32 bytes of the head dimension
-              const uint64_t a = q_desc + (k >> 2) * (C::Q_SPAN >> 4) + 2 * (k & 3);
-              const uint64_t b = k_desc + (k >> 2) * (C::KV_SPAN >> 4) + 2 * (k & 3);
-              if (FP8) mma_f8_ss(d, a, b, idesc_qk, k != 0);
-              else mma_f16_ss(d, a, b, idesc_qk, k != 0);
-            }
-            tc_commit(s_full((J + j) & 1));
-            tc_commit(k_empty(st));
-          }
-        };
-        issue_qk(0);
-        if (s.tiles > 1) issue_qk(1);
-        // O of the segment before has been read
-        if (n_seg > 0) ok = ok && mbar_wait_warp(o_free, (n_seg - 1) & 1, p.status, WK_ERR_TIMEOUT_TMEM);
-        for (int j = 0; ok && j < s.tiles; ++j) {
-          const int st = (J + j) % ST, buf = (J + j) & 1;
-          ok = mbar_wait_warp(p_full(buf), ((J + j) >> 1) & 1, p.status, WK_ERR_TIMEOUT_P);
-          if (!FP8) ok = ok && mbar_wait_warp(v_full(st), ((J + j) / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+          const uint32_t ph = ((J + j) / ST) & 1;
+          const int key0 = (tile0 + j) * X_KEYS;
+          ok = mbar_wait(k_empty(st), ph ^ 1, p.status, WK_ERR_TIMEOUT_EMPTY);
           if (!ok) break;
-          tc_fence_after();
-          const uint64_t v_desc = smem_desc_sw128(
-              FP8 ? smem + C::V16_AT + buf * C::V16_BYTES : smem + C::V_AT + st * C::K_BYTES, C::KV_SPAN, 1024);
-          if (mine) {
-#pragma unroll
-            for (int k = 0; k < X_KEYS / 16; ++k)
-              mma_f16_ts(tmem + X_O_COL, tmem + buf * X_S_COLS + 8 * k, v_desc + 128 * k, idesc_pv, (j | k) != 0);
-            if (!FP8) tc_commit(v_empty(st));
-            if (j == s.tiles - 1) tc_commit(o_full);
-          }
-          if (j + 2 < s.tiles) issue_qk(j + 2);
-        }
-        __syncwarp();
-      } else {
-        const int quad = warp & 3, grp = (warp - 2) >> 2;
-        const int t = threadIdx.x - 64;
-        const int r = quad * 32 + lane;  // row of the tile = lane of tensor memory
-        const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-        const uint32_t s_tmem = tmem + lane_addr + grp * X_S_COLS;
-        {
-          // the unit's rows of Q, swizzled like a TMA tile; every product that read the last ones has completed
-          constexpr int PIECES = DH * C::SIZE / 16;
-          for (int x = t; x < s.rows * PIECES; x += X_SOFTMAX) {
-            const int row = x / PIECES, c = x % PIECES;
-            int m = s.row0 + row, b = s.b;
-            if (!s.own) b = m / p.rows_own, m -= b * p.rows_own;
-            const int g = m / p.Nq, n = m - g * p.Nq;
-            const uint8_t* src = p.q + b * p.q_strides[0] + (s.h * p.group + g) * p.q_strides[1] + n * p.q_strides[2] + 16 * c;
-            cp_async16(smem + C::Q_AT + (c >> 3) * C::Q_SPAN + row * 128 + (((c & 7) ^ (row & 7)) << 4), src);
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          fence_proxy_async_smem();
-          mbar_arrive(q_full);
-        }
-        const bool live = r < s.rows, warp_live = quad * 32 < s.rows;
-        int b = s.b, limit = s.keys - 1;  // last key of the range that the row sees
-        {
-          int m = s.row0 + min(r, s.rows - 1);
-          if (!s.own) b = m / p.rows_own, m -= b * p.rows_own;
-          if (p.causal) {
-            const int used = s.own ? s.keys : p.seqused ? max(0, min(p.S, p.seqused[b])) : p.S;
-            limit = min(limit, (s.own ? 0 : p.P) + m % p.Nq + used - p.Nq);
-          }
-        }
-        float beta = p.scale_log2, v_scale = 1.f;
-        if (FP8) {
-          beta *= p.q_descale[b * p.Hkv + s.h] * (s.own ? p.k_descale[b * p.Hkv + s.h] : p.kp_descale[s.h]);
-          v_scale = s.own ? p.v_descale[b * p.Hkv + s.h] : p.vp_descale[s.h];
-        }
-        const uint32_t x_ref = smem + C::X_AT + r * 4;
-        auto x_group = [&](int g) { return x_ref + (1 + 2 * g) * X_ROWS * 4; };
-        const int64_t slot = s.slot + r;
-        float m_ref = pass && live ? p.part_top[slot] : -INFINITY, top = -INFINITY, l = 0.f;
-        bool met = false;
-        for (int j = (J + grp) & 1; j < s.tiles; j += 2) {
-          const int tile = J + j;
-          ok = ok && mbar_wait_warp(s_full(grp), (tile >> 1) & 1, p.status, WK_ERR_TIMEOUT_MMA);
+          mbar_expect_tx(k_full(st), C::K_BYTES);
+          for (int c = 0; c < C::SPANS; ++c)
+            tma_load_4d(smem + C::K_AT + st * C::K_BYTES + c * C::KV_SPAN, &map_k, k_full(st), 64 * c, key0, h, b);
+          ok = mbar_wait(v_empty(st), ph ^ 1, p.status, WK_ERR_TIMEOUT_EMPTY);
           if (!ok) break;
-          tc_fence_after();
-          const int key0 = (s.tile0 + j) * X_KEYS;
-          const bool masked = __any_sync(0xffffffffu, key0 + X_KEYS - 1 > limit);
-          const int last = limit - key0;  // columns beyond it are masked
-          if (j == 0 && pass == 0) {
-            float m = -INFINITY;
-            if (warp_live) {
-#pragma unroll 1
-              for (int c = 0; c < 2; ++c) {
-                uint32_t raw[32];
-                tmem_ld32(s_tmem + c * 32, raw);
-                tc_wait_ld();
-                if (masked) {
+          mbar_expect_tx(v_full(st), C::K_BYTES);
+          for (int c = 0; c < C::SPANS; ++c)
+            tma_load_4d(smem + C::V_AT + st * C::K_BYTES + c * C::KV_SPAN, &map_v, v_full(st), 64 * c, key0, h, b);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      const bool mine = elect_one();
+      constexpr uint32_t idesc_qk = FP8 ? make_idesc(0, 0, 0, 0, X_ROWS, X_KEYS) : make_idesc(1, 1, 0, 0, X_ROWS, X_KEYS);
+      constexpr uint32_t idesc_pv = make_idesc(1, 1, 0, 1, X_ROWS, DH);
+      const uint64_t q_desc = smem_desc_sw128(smem + C::Q_AT, 16, 1024);
+      if (pass == 0) ok = mbar_wait_warp(q_full, 0, p.status, WK_ERR_TIMEOUT_LOAD);
+      // the tensor pipe runs in issue order: the scores also wait for the product that last read their buffer
+      auto issue_qk = [&](int j) {
+        const int st = (J + j) % ST;
+        ok = ok && mbar_wait_warp(k_full(st), ((J + j) / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t k_desc = smem_desc_sw128(smem + C::K_AT + st * C::K_BYTES, 16, 1024);
+        const uint32_t d = tmem + ((J + j) & 1) * X_S_COLS;
+        if (mine) {
 #pragma unroll
-                  for (int x = 0; x < 32; ++x)
-                    if (c * 32 + x > last) raw[x] = 0xff800000u;
-                }
-                m = fmaxf(m, block_max(raw) * beta);
-              }
-            }
-            m_ref = m;
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_ref), "f"(m) : "memory");
+          for (int k = 0; k < DH * C::SIZE / 32; ++k) {  // 32 bytes of the head dimension
+            const uint64_t x = q_desc + (k >> 2) * (C::Q_SPAN >> 4) + 2 * (k & 3);
+            const uint64_t y = k_desc + (k >> 2) * (C::KV_SPAN >> 4) + 2 * (k & 3);
+            if (FP8) mma_f8_ss(d, x, y, idesc_qk, k != 0);
+            else mma_f16_ss(d, x, y, idesc_qk, k != 0);
           }
-          if (!met) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            met = true;
-            if (j != 0 && pass == 0) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(m_ref) : "r"(x_ref) : "memory");
-          }
-          const int st = tile % ST;
-          if (FP8) {
-            // this tile of V to bf16: a thread takes half a row.  Rows behind the last key become zeros, whatever the cache
-            // holds there: 0 . V has to be 0.
-            ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-            if (!ok) break;
-            constexpr int HALF = DH / 32;  // 16-byte pieces of half a row
-            const int row = r >> 1;
-            const uint32_t src = smem + C::V_AT + st * C::K_BYTES + row * 128;
-            const uint32_t dst = smem + C::V16_AT + grp * C::V16_BYTES + row * 128;
-            const bool there = key0 + row < s.keys;
+          tc_commit(s_full((J + j) & 1));
+          tc_commit(k_empty(st));
+        }
+      };
+      issue_qk(0);
+      if (tiles > 1) issue_qk(1);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int st = (J + j) % ST, buf = (J + j) & 1;
+        ok = mbar_wait_warp(p_full(buf), ((J + j) >> 1) & 1, p.status, WK_ERR_TIMEOUT_P);
+        if (!FP8) ok = ok && mbar_wait_warp(v_full(st), ((J + j) / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v_desc = smem_desc_sw128(
+            FP8 ? smem + C::V16_AT + buf * C::V16_BYTES : smem + C::V_AT + st * C::K_BYTES, C::KV_SPAN, 1024);
+        if (mine) {
 #pragma unroll
-            for (int c = 0; c < HALF; ++c) {
-              const int piece = (r & 1) * HALF + c;
-              uint32_t w[4], o[8];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                           : "r"(src + ((piece ^ (row & 7)) << 4)));
+          for (int k = 0; k < X_KEYS / 16; ++k)
+            mma_f16_ts(tmem + X_O_COL, tmem + buf * X_S_COLS + 8 * k, v_desc + 128 * k, idesc_pv, (j | k) != 0);
+          if (!FP8) tc_commit(v_empty(st));
+          if (j == tiles - 1) tc_commit(o_full);
+        }
+        if (j + 2 < tiles) issue_qk(j + 2);
+      }
+      __syncwarp();
+    } else {
+      const int quad = warp & 3, grp = (warp - 2) >> 2;
+      const int t = threadIdx.x - 64;
+      const int r = quad * 32 + lane;  // row of the tile = lane of tensor memory
+      const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+      const uint32_t s_tmem = tmem + lane_addr + grp * X_S_COLS;
+      const bool live = r < rows, warp_live = quad * 32 < rows;
+      int seq = b, limit = keys - 1;  // the row's sequence, the last key of the range that it sees
+      int m = row0 + min(r, rows - 1);
+      if (!OWN) seq = m / p.rows_own, m -= seq * p.rows_own;
+      const int g = m / p.Nq, n = m - g * p.Nq;
+      if (p.causal) limit = min(limit, OWN ? n + keys - p.Nq : p.P + n + own_keys(p, seq) - p.Nq);
+      if (pass == 0) {
+        // The unit's rows of Q, swizzled like a TMA tile, eight lanes to 128 bytes of a row.
+        const int64_t from = seq * p.q_strides[0] + (h * p.group + g) * p.q_strides[1] + n * p.q_strides[2];
+        if (grp == 0) asm volatile("st.shared.b64 [%0], %1;" ::"r"(smem + C::ROW_AT + r * 8), "l"(from) : "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        constexpr int PIECES = DH * C::SIZE / 16, LANES = PIECES < 8 ? PIECES : 8;
+        const int c = t % LANES;
+        for (int row = t / LANES; row < rows; row += X_SOFTMAX / LANES) {
+          int64_t at;
+          asm volatile("ld.shared.b64 %0, [%1];" : "=l"(at) : "r"(smem + C::ROW_AT + row * 8) : "memory");
 #pragma unroll
-              for (int x = 0; x < 4; ++x) e4m3x4_to_bf16(there ? w[x] : 0u, o[2 * x], o[2 * x + 1]);
-              const uint32_t to = dst + (piece >> 2) * C::KV_SPAN;
-              const int at = (2 * piece) & 7;
-              sts128(to + ((at ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
-              sts128(to + (((at + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
-            }
-            mbar_arrive(v_empty(st));
-            fence_proxy_async_smem();
-          } else if (key0 + X_KEYS > s.keys) {
-            ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-            if (!ok) break;
-            const int row = r >> 1;
-            if (key0 + row >= s.keys && (r & 1) < C::V_SPANS) {
-              const uint32_t at = smem + C::V_AT + st * C::K_BYTES + (r & 1) * C::KV_SPAN + row * 128;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) sts128(at + 16 * c, 0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
+          for (int span = 0; span < C::SPANS; ++span)
+            cp_async(smem + C::Q_AT + span * C::Q_SPAN + row * 128 + ((c ^ (row & 7)) << 4), p.q + at + span * 128 + 16 * c, 16);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      }
+      float beta = p.scale_log2, v_scale = 1.f;
+      if (FP8) {
+        beta *= __ldcg(p.q_descale + seq * p.Hkv + h) * __ldcg(OWN ? p.k_descale + seq * p.Hkv + h : p.kp_descale + h);
+        v_scale = __ldcg(OWN ? p.v_descale + seq * p.Hkv + h : p.vp_descale + h);
+      }
+      const uint32_t x_ref = smem + C::X_AT + r * 4;
+      auto x_group = [&](int g) { return x_ref + (1 + 2 * g) * X_ROWS * 4; };
+      float top = -INFINITY, l = 0.f;
+      bool met = false;
+      for (int j = (J + grp) & 1; j < tiles; j += 2) {
+        const int tile = J + j;
+        ok = ok && mbar_wait_warp(s_full(grp), (tile >> 1) & 1, p.status, WK_ERR_TIMEOUT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = (tile0 + j) * X_KEYS;
+        const bool masked = __any_sync(0xffffffffu, key0 + X_KEYS - 1 > limit);
+        const int last = limit - key0;  // columns beyond it are masked
+        if (j == 0 && pass == 0) {
+          float x = -INFINITY;
           if (warp_live) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 2; ++c) {
               uint32_t raw[32];
               tmem_ld32(s_tmem + c * 32, raw);
               tc_wait_ld();
               if (masked) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                  if (c * 32 + x > last) raw[x] = 0xff800000u;
+                for (int i = 0; i < 32; ++i)
+                  if (c * 32 + i > last) raw[i] = 0xff800000u;
               }
-              top = fmaxf(top, block_max(raw) * beta);
-              const float bias = m_ref > -INFINITY ? -m_ref : 0.f;
-              uint32_t w[16];
-              float sum;
-              softmax_block(raw, beta, bias, w, sum);
-              l += sum;
-              uint32_t lo[8], hi[8];
-#pragma unroll
-              for (int x = 0; x < 8; ++x) lo[x] = w[x], hi[x] = w[8 + x];
-              tmem_st8(s_tmem + c * 16, lo);
-              tmem_st8(s_tmem + c * 16 + 8, hi);
+              x = fmaxf(x, block_max(raw) * beta);
             }
-            tc_wait_st();
           }
-          tc_fence_before();
-          mbar_arrive(p_full(grp));
+          m_ref = x;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_ref), "f"(x) : "memory");
         }
-        if (!met) {  // no tile, or a wait gave up: the other group waits for the meeting all the same
+        if (!met) {
           asm volatile("bar.sync 1, 256;" ::: "memory");
-          if (pass == 0) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(m_ref) : "r"(x_ref) : "memory");
+          met = true;
+          if (j != 0 && pass == 0) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(m_ref) : "r"(x_ref) : "memory");
         }
-        ok = ok && mbar_wait_warp(o_full, n_seg & 1, p.status, WK_ERR_TIMEOUT_MMA);
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_group(grp)), "f"(l) : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_group(grp) + X_ROWS * 4), "f"(top) : "memory");
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        float l2, top2;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(l2) : "r"(x_group(grp ^ 1)) : "memory");
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(top2) : "r"(x_group(grp ^ 1) + X_ROWS * 4) : "memory");
-        l += l2;
-        top = fmaxf(top, top2);
-        if (ok) {
-          tc_fence_after();
-          const float inv = l > 0.f ? v_scale / l : l == l ? 0.f : l;  // NaN stays
-          float* dst = p.part + slot * DH + grp * (DH / 2);
-          if (warp_live) {
+        const int st = tile % ST;
+        if (FP8) {
+          // this tile of V to bf16: a thread takes half a row.  Rows behind the last key become zeros, whatever the cache
+          // holds there: 0 . V has to be 0.
+          ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+          if (!ok) break;
+          constexpr int HALF = DH / 32;  // 16-byte pieces of half a row
+          const int row = r >> 1;
+          const uint32_t src = smem + C::V_AT + st * C::K_BYTES + row * 128;
+          const uint32_t dst = smem + C::V16_AT + grp * C::V16_BYTES + row * 128;
+          const bool there = key0 + row < keys;
 #pragma unroll
-            for (int c = 0; c < DH / 64; ++c) {
-              uint32_t v[32];
-              tmem_ld32(tmem + lane_addr + X_O_COL + grp * (DH / 2) + c * 32, v);
-              tc_wait_ld();
-              if (live)
+          for (int c = 0; c < HALF; ++c) {
+            const int piece = (r & 1) * HALF + c;
+            uint32_t w[4], o[8];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(src + ((piece ^ (row & 7)) << 4)));
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                  reinterpret_cast<float4*>(dst + c * 32)[x] =
-                      make_float4(__uint_as_float(v[4 * x]) * inv, __uint_as_float(v[4 * x + 1]) * inv,
-                                  __uint_as_float(v[4 * x + 2]) * inv, __uint_as_float(v[4 * x + 3]) * inv);
-              __syncwarp();
+            for (int x = 0; x < 4; ++x) e4m3x4_to_bf16(there ? w[x] : 0u, o[2 * x], o[2 * x + 1]);
+            const uint32_t to = dst + (piece >> 2) * C::KV_SPAN;
+            const int at = (2 * piece) & 7;
+            sts128(to + ((at ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+            sts128(to + (((at + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
+          }
+          mbar_arrive(v_empty(st));
+          fence_proxy_async_smem();
+        } else if (key0 + X_KEYS > keys) {
+          ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+          if (!ok) break;
+          const int row = r >> 1;
+          if (key0 + row >= keys && (r & 1) < C::V_SPANS) {
+            const uint32_t at = smem + C::V_AT + st * C::K_BYTES + (r & 1) * C::KV_SPAN + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) sts128(at + 16 * c, 0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        if (warp_live) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t raw[32];
+            tmem_ld32(s_tmem + c * 32, raw);
+            tc_wait_ld();
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (c * 32 + i > last) raw[i] = 0xff800000u;
             }
+            top = fmaxf(top, block_max(raw) * beta);
+            const float bias = m_ref > -INFINITY ? -m_ref : 0.f;
+            uint32_t w[16];
+            float sum;
+            softmax_block(raw, beta, bias, w, sum);
+            l += sum;
+            uint32_t lo[8], hi[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) lo[i] = w[i], hi[i] = w[8 + i];
+            tmem_st8(s_tmem + c * 16, lo);
+            tmem_st8(s_tmem + c * 16 + 8, hi);
           }
-          if (live && grp == 0) {
-            p.part_lse[slot] = l == 0.f ? -INFINITY : m_ref + log2f(l);
-            p.part_top[slot] = top;
-            if (pass == 0 && top - m_ref > X_MAX_EXP)
-              atomicOr(const_cast<uint32_t*>(flags) + flag / 32, 1u << (flag % 32));
-          }
+          tc_wait_st();
         }
         tc_fence_before();
-        mbar_arrive(o_free);
-        __syncwarp();
+        mbar_arrive(p_full(grp));
       }
-      J += s.tiles;
-      ++n_seg;
+      if (!met) {  // no tile, or a wait gave up: the other group waits for the meeting all the same
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (pass == 0) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(m_ref) : "r"(x_ref) : "memory");
+      }
+      ok = ok && mbar_wait_warp(o_full, pass, p.status, WK_ERR_TIMEOUT_MMA);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_group(grp)), "f"(l) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(x_group(grp) + X_ROWS * 4), "f"(top) : "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float l2, top2;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(l2) : "r"(x_group(grp ^ 1)) : "memory");
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(top2) : "r"(x_group(grp ^ 1) + X_ROWS * 4) : "memory");
+      l += l2;
+      top = fmaxf(top, top2);
+      far = ok && live && pass == 0 && top - m_ref > X_MAX_EXP;
+      inv_row = l > 0.f ? v_scale / l : l == l ? 0.f : l;  // NaN stays
+      lse_row = l == 0.f ? -INFINITY : m_ref + log2f(l);
+      if (pass == 0) m_ref = top;  // for the second pass
+      tc_fence_after();
     }
-    __syncthreads();  // flags and largest scores are there
-    if (pass == 0) {
-      bool any = false;
-      for (int i = 0; i < X_FLAGS / 32; ++i) any |= flags[i] != 0;
-      if (!any) break;
-    }
+    if (!__syncthreads_or(far) || pass) break;
   }
-  tc_fence_before();
-  __syncthreads();
+
+  // ---- this CTA's part to shared memory: every tile and product has been used
+  uint8_t* part = smem_raw + (smem - smem_u32(smem_raw));  // [row][DH + X_PAD]
+  if (warp >= 2) {
+    const int quad = warp & 3, grp = (warp - 2) >> 2, r = quad * 32 + lane;
+    const uint32_t o_tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + X_O_COL + grp * (DH / 2);
+    if (quad * 32 < rows) {
+#pragma unroll
+      for (int c = 0; c < DH / 64; ++c) {
+        uint32_t v[32];
+        if (tiles > 0) {
+          tmem_ld32(o_tmem + c * 32, v);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          reinterpret_cast<float4*>(part + r * (DH + X_PAD) * 4)[grp * (DH / 8) + c * 8 + i] =
+              make_float4(__uint_as_float(v[4 * i]) * inv_row, __uint_as_float(v[4 * i + 1]) * inv_row,
+                          __uint_as_float(v[4 * i + 2]) * inv_row, __uint_as_float(v[4 * i + 3]) * inv_row);
+      }
+    }
+    if (grp == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + C::X_AT + r * 4), "f"(lse_row) : "memory");
+    tc_fence_before();
+  }
+  const bool meet = !OWN && p.cluster > 1;
+  if (meet) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, X_TMEM_COLS);
   }
+  const bool final = !OWN && p.splits == 1;
+  if (beside) pdl_wait();  // the parts of own keys are there, and nothing that comes after this kernel starts before them
+
+  // ---- the rows congruent to this CTA's rank: first what each member's part and the own keys' parts count, one thread to
+  // a row, then the sums, a warp or half of one to a row
+  const int rank = OWN ? 0 : blockIdx.x % p.cluster, members = OWN ? 1 : p.cluster;
+  const int mine = rank < rows ? (rows - rank + members - 1) / members : 0;
+  RowEnd* ends = reinterpret_cast<RowEnd*>(part + C::PART_BYTES);
+  for (int i = threadIdx.x; i < mine; i += X_THREADS) {
+    const int r = i * members + rank;
+    const uint32_t stat = smem + C::X_AT + r * 4;
+    RowEnd e;
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int k = 0; k < X_CLUSTER; ++k) {
+      e.weight[k] = -INFINITY;
+      if (k < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(e.weight[k]) : "r"(meet ? mapa(stat, k) : stat));
+    }
+#pragma unroll
+    for (int k = 0; k < X_CLUSTER; ++k) top = fmaxf(top, e.weight[k]);
+    int seq = b, own = row0 + r;
+    if (!OWN) seq = own / p.rows_own, own -= seq * p.rows_own;
+    e.parts = 0;
+    if (final && p.S) {
+      const OwnParts parts(p, seq, h, own);
+      e.first = parts.first, e.parts = parts.count;
+      for (int k = 0; k < parts.count; ++k) top = fmaxf(top, __ldcg(p.part_lse + parts.first + k * parts.distance));
+      for (int k = 0; k < parts.count; ++k) {
+        const float lse = __ldcg(p.part_lse + parts.first + k * parts.distance);
+        total += lse == -INFINITY ? 0.f : exp2f(lse - top);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < X_CLUSTER; ++k) {
+      e.weight[k] = e.weight[k] == -INFINITY ? 0.f : exp2f(e.weight[k] - top);
+      total += e.weight[k];
+    }
+    const bool empty = total == 0.f;
+    e.top = top, e.inv = empty ? 0.f : 1.f / total;
+    const float lse = empty ? INFINITY : top + log2f(total);
+    if (final) {
+      const int g = own / p.Nq, n = own - g * p.Nq, head = h * p.group + g;
+      e.to = seq * p.out_strides[0] + head * p.out_strides[1] + n * p.out_strides[2];
+      if (p.lse) p.lse[seq * p.lse_strides[0] + head * p.lse_strides[1] + n] = p.lse_natural ? lse * 0.6931471805599453f : lse;
+    } else {
+      e.to = OWN ? own_slot_of(p, blockIdx.x, 0) + r : static_cast<int64_t>(blockIdx.x / p.cluster) * X_ROWS + r;
+      p.part_lse[e.to] = empty ? -INFINITY : lse;
+    }
+    ends[i] = e;
+  }
+  __syncthreads();
+  constexpr int QUADS = DH / 4;
+  for (int i = threadIdx.x; i < mine * QUADS; i += X_THREADS) {
+    const int c = i % QUADS, r = i / QUADS * members + rank;
+    const RowEnd& e = ends[i / QUADS];
+    const uint32_t at = smem + r * (DH + X_PAD) * 4 + c * 16;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4& v) {
+      o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+    };
+    for (int k = 0; k < e.parts; ++k) {
+      const int64_t slot = e.first + k * p.own_slot;
+      const float lse = __ldcg(p.part_lse + slot);
+      add(lse == -INFINITY ? 0.f : exp2f(lse - e.top), __ldcg(reinterpret_cast<const float4*>(p.part + slot * DH) + c));
+    }
+    for (int k0 = 0; k0 < members; k0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < members)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
+                       : "r"(meet ? mapa(at, k0 + k) : at));
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) add(e.weight[k0 + k], v[k]);
+    }
+    o.x *= e.inv, o.y *= e.inv, o.z *= e.inv, o.w *= e.inv;
+    if (final)
+      *reinterpret_cast<uint2*>(p.out + e.to + 4 * c) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
+    else
+      reinterpret_cast<float4*>(p.part + e.to * DH)[c] = o;
+  }
+  __syncwarp();
+  if (meet) cluster_sync();  // nobody leaves while its part may still be read
 }
 
-// Adds up the segments of every row.  WARPS warps for a row, a row of a CTA's 8 / WARPS.
-template <int DH, int WARPS>
+// ---- own keys of sequences with few rows ---------------------------------------------------------------------------
+// A unit is up to 16 rows of one (sequence, KV head) and its own keys, in steps of KEYS; it weighs one more than its steps,
+// for its start and end.  All units form a line that is cut into as many pieces as there are warps; a warp goes through its
+// piece by itself, its fetches three steps ahead and on into the next units, and leaves a part of every unit.
+
+// Exclusive sums of the sequences' weights, by the whole CTA; `cum` is in shared or global memory.
+template <int KEYS>
+__device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int* warp_sums) {
+  constexpr int THREADS = 32 * Y_WARPS;
+  const int per = (p.B + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(p.B, b0 + per);
+  auto weight = [&](int b) { return (own_keys(p, b) + KEYS - 1) / KEYS + Y_START; };
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += weight(b);
+  int scan = sum;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
+  for (int i = 1; i < 32; i *= 2) {
+    const int other = __shfl_up_sync(0xffffffffu, scan, i);
+    if (lane >= i) scan += other;
+  }
+  if (lane == 31) warp_sums[warp] = scan;
+  __syncthreads();
+  int at = scan - sum;
+  for (int w = 0; w < warp; ++w) at += warp_sums[w];
+  for (int b = b0; b < b1; ++b) {
+    cum[b] = at;
+    at += weight(b);
+  }
+  if (b1 == p.B && b0 < p.B) cum[p.B] = at;
+  __syncthreads();
+}
+
+template <bool FP8, int DH>
+struct OwnWalker {
+  int x, x1;           // where in the line, end of the piece
+  int b, h, block, u;  // sequence, KV head, 16 rows; u = h . blocks + block
+  int weight, nk, step, end, base;
+  __device__ __forceinline__ void open(const PrefixParams& p, const int* cum) {
+    weight = cum[b + 1] - cum[b];
+    nk = own_keys(p, b);
+  }
+  // Steps of the piece in the unit that starts at `at`.
+  __device__ __forceinline__ void range(int at) {
+    base = at;
+    step = max(0, x - base - Y_START);
+    end = min(weight, x1 - base) - Y_START;
+  }
+  __device__ __forceinline__ OwnWalker(const PrefixParams& p, const Pieces& l, const int* cum, int blocks, int piece) {
+    x = x1 = 0;
+    if (piece >= l.G) return;
+    x = l.start(piece), x1 = l.start(piece + 1);
+    const int per_seq = p.Hkv * blocks;
+    int lo = 0, hi = p.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (cum[mid] * per_seq <= x) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    open(p, cum);
+    const int first = cum[b] * per_seq;
+    u = (x - first) / weight;
+    h = u / blocks, block = u - h * blocks;
+    range(first + u * weight);
+    if (step >= end) next(p, cum, blocks);
+  }
+  __device__ __forceinline__ bool here() const { return x < x1; }
+  // To the next unit that this piece has part in.
+  __device__ __forceinline__ void next(const PrefixParams& p, const int* cum, int blocks) {
+    do {
+      x = base + weight;  // where the next unit starts
+      if (x >= x1) return;
+      ++u;
+      if (++block == blocks) block = 0, ++h;
+      if (u == p.Hkv * blocks) {
+        u = h = 0, ++b;
+        open(p, cum);
+      }
+      range(x);
+    } while (step >= end);  // nothing of the unit but its start is in the piece, or it has no keys
+  }
+};
+
+template <bool FP8, int DH>
+__global__ void __launch_bounds__(32 * Y_WARPS, 2)
+attn_prefix_own_kernel(const __grid_constant__ PrefixParams p) {
+  using C = RowsCfg<FP8, DH>;
+  extern __shared__ __align__(16) uint8_t ring_mem[];
+  __shared__ int cum_mem[Y_CUM + 1], warp_sums[Y_WARPS];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  pdl_wait();
+  // the prefix kernel runs beside this one and reads what was written before it: it may start only now
+  pdl_launch_dependents();
+  // every CTA writes the same counts where they do not fit shared memory; those that add the parts read them from there
+  int* cum = p.B <= Y_CUM ? cum_mem : p.cum;
+  sum_weights<C::KEYS>(p, cum, warp_sums);
+  if (blockIdx.x == 0 && cum != p.cum)
+    for (int i = threadIdx.x; i <= p.B; i += 32 * Y_WARPS) p.cum[i] = cum[i];
+  const int blocks = p.blocks_own, per_seq = p.Hkv * blocks;
+  const Pieces line(cum[p.B] * per_seq, p.pieces);
+  const int piece = blockIdx.x * Y_WARPS + warp;
+  const uint32_t ring = smem_u32(ring_mem) + warp * Y_STAGES * C::STAGE_BYTES;
+
+  OwnWalker<FP8, DH> now(p, line, cum, blocks, piece), ahead = now;
+  const uint8_t *k_base = nullptr, *v_base = nullptr;
+  auto start = [&]() {
+    k_base = p.k + ahead.b * p.k_strides[0] + ahead.h * p.k_strides[1] + t * 16;
+    v_base = p.v + ahead.b * p.v_strides[0] + ahead.h * p.v_strides[1] + g * C::V_PIECE;
+  };
+  auto fetch = [&](int stage) {
+    if (ahead.here()) {
+      const uint32_t ks = ring + stage * C::STAGE_BYTES + lane * 16;
+      const uint32_t vs = ring + stage * C::STAGE_BYTES + C::K_BYTES + lane * C::V_PIECE;
+      const int key0 = ahead.step * C::KEYS;
+#pragma unroll
+      for (int j = 0; j < C::N8; ++j) {  // keys beyond the last one are masked: any valid row will do
+        const uint8_t* src = k_base + min(key0 + 8 * j + g, ahead.nk - 1) * p.k_strides[2];
+#pragma unroll
+        for (int i = 0; i < C::K_PIECES; ++i) cp_async(ks + (j * C::K_PIECES + i) * 512, src + 64 * i, 16);
+      }
+#pragma unroll
+      for (int j = 0; j < C::KEYS / 4; ++j) {
+        const uint8_t* src = v_base + min(key0 + 8 * (j / 2) + 2 * t + (j & 1), ahead.nk - 1) * p.v_strides[2];
+#pragma unroll
+        for (int i = 0; i < C::V_PIECES; ++i)
+          cp_async(vs + (j * C::V_PIECES + i) * (32 * C::V_PIECE), src + 8 * C::V_PIECE * i, C::V_PIECE);
+      }
+      if (++ahead.step == ahead.end) {
+        ahead.next(p, cum, blocks);
+        if (ahead.here()) start();
+      }
+    }
+    cp_async_commit();
+  };
+  if (ahead.here()) start();
+  for (int i = 0; i < Y_STAGES; ++i) fetch(i);
+
+  int stage = 0;
+  for (; now.here(); now.next(p, cum, blocks)) {
+    const int row0 = now.block * R_ROWS, sc = now.b * p.Hkv + now.h, unit = now.b * per_seq + now.u;
+    uint4 q[2][C::K_PIECES];
+    int limit[2], first_limit = now.nk - 1;  // last visible keys of the thread's two rows, and of all rows of the unit
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = min(row0 + g + 8 * i, p.rows_own - 1), n = r % p.Nq;
+      const uint8_t* src = p.q + now.b * p.q_strides[0] + (now.h * p.group + r / p.Nq) * p.q_strides[1] + n * p.q_strides[2] + t * 16;
+#pragma unroll
+      for (int j = 0; j < C::K_PIECES; ++j) q[i][j] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * j));
+      limit[i] = p.causal ? min(now.nk - 1, n + now.nk - p.Nq) : now.nk - 1;
+    }
+    if (p.causal) first_limit = min(first_limit, now.nk - p.Nq);  // of query 0, whether it is among them or not
+    float beta = p.scale_log2, v_scale = 1.f;
+    if (FP8) beta *= __ldcg(p.q_descale + sc) * __ldcg(p.k_descale + sc), v_scale = __ldcg(p.v_descale + sc);
+
+    float o[C::NT][4];
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int step = now.step; step < now.end; ++step) {
+      cp_async_wait<Y_STAGES - 1>();
+      rows_step<FP8, DH>(ring + stage * C::STAGE_BYTES + lane * 16,
+                         ring + stage * C::STAGE_BYTES + C::K_BYTES + lane * C::V_PIECE, q, beta, step * C::KEYS, first_limit,
+                         limit, t, o, m, l, top);
+      // the stage's own reads are done (their values have been used): refill it
+      fetch(stage);
+      if (++stage == Y_STAGES) stage = 0;
+    }
+
+    // ---- this warp's part: O / l and the log-sum-exp.  Column tile j of the MMAs holds element j % V_ELEMS of piece
+    // j / V_ELEMS of the eight lanes that share a V row.
+    const int64_t slot = own_slot_of(p, unit, piece);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      const int r = g + 8 * i;
+      if (row0 + r < p.rows_own) {
+        const float inv = l[i] > 0.f ? v_scale / l[i] : l[i] == l[i] ? 0.f : l[i];
+        float* dst = p.part + (slot + r) * DH;
+#pragma unroll
+        for (int j = 0; j < C::NT; j += 4) {
+          float* at = dst + (j / C::V_ELEMS) * (8 * C::V_ELEMS) + 2 * t * C::V_ELEMS + j % C::V_ELEMS;
+          *reinterpret_cast<float4*>(at) = make_float4(o[j][2 * i] * inv, o[j + 1][2 * i] * inv, o[j + 2][2 * i] * inv,
+                                                       o[j + 3][2 * i] * inv);
+          *reinterpret_cast<float4*>(at + C::V_ELEMS) = make_float4(
+              o[j][2 * i + 1] * inv, o[j + 1][2 * i + 1] * inv, o[j + 2][2 * i + 1] * inv, o[j + 3][2 * i + 1] * inv);
+        }
+        if (t == 0) p.part_lse[slot + r] = l[i] == 0.f ? -INFINITY : m[i] - C::P_SHIFT + log2f(l[i]);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// Adds up the parts of every row: a warp for a row, as many columns to a lane as there are.
+template <int DH>
 __global__ void __launch_bounds__(256)
 attn_prefix_combine_kernel(const __grid_constant__ PrefixParams p) {
-  constexpr int COLS = DH / 32;  // per lane
-  __shared__ float part_o[8][DH], part_m[8], part_l[8];
+  constexpr int COLS = DH / 32;
+  struct alignas(4 * COLS) Vec {
+    float x[COLS];
+  };
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int row = blockIdx.x * (8 / WARPS) + warp / WARPS, share = warp % WARPS;
-  const int rows = p.B * p.Hq * p.Nq;
-  const bool live = row < rows;
-  int b = 0, head = 0, n = 0;
-  float m = -INFINITY, l = 0.f, o[COLS];
+  const int lane = threadIdx.x % 32, row = blockIdx.x * 8 + threadIdx.x / 32;
+  if (row >= p.Hkv * p.rows_all) return;
+  const int h = row / p.rows_all, stacked = row - h * p.rows_all, b = stacked / p.rows_own, own = stacked - b * p.rows_own;
+  const OwnParts parts(p, b, h, own);
+  const int splits = p.tiles_p ? p.splits : 0, all = splits + parts.count;
+  const int64_t first = static_cast<int64_t>(h * p.blocks_p + stacked / X_ROWS) * p.splits * X_ROWS + stacked % X_ROWS;
+  auto slot_of = [&](int c) { return c < splits ? first + c * X_ROWS : parts.first + static_cast<int64_t>(c - splits) * parts.distance; };
+  float top = -INFINITY;
+  for (int c = lane; c < all; c += 32) top = fmaxf(top, __ldcg(p.part_lse + slot_of(c)));
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+  float total = 0.f, o[COLS];
 #pragma unroll
   for (int i = 0; i < COLS; ++i) o[i] = 0.f;
-  auto add = [&](int64_t slot) {
-    const float x = __ldcg(p.part_lse + slot);
-    float v[COLS];
-    const float* src = p.part + slot * DH + lane * COLS;
+#pragma unroll 4
+  for (int c = 0; c < all; ++c) {
+    const int64_t slot = slot_of(c);
+    const float lse = __ldcg(p.part_lse + slot), w = lse == -INFINITY ? 0.f : exp2f(lse - top);
+    Vec v;
     if (COLS == 4) {
-      const float4 w = __ldcg(reinterpret_cast<const float4*>(src));
-      v[0] = w.x, v[1] = w.y, v[COLS - 2] = w.z, v[COLS - 1] = w.w;
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part + slot * DH) + lane);
+      v.x[0] = y.x, v.x[1] = y.y, v.x[COLS - 2] = y.z, v.x[COLS - 1] = y.w;
     } else {
-      const float2 w = __ldcg(reinterpret_cast<const float2*>(src));
-      v[0] = w.x, v[1] = w.y;
+      const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part + slot * DH) + lane);
+      v.x[0] = y.x, v.x[1] = y.y;
     }
-    const float top = fmaxf(m, x);
-    const float f = m > -INFINITY ? exp2f(m - top) : 0.f, g = x == -INFINITY ? 0.f : exp2f(x - top);
-    l = l * f + g;
+    total += w;
 #pragma unroll
-    for (int i = 0; i < COLS; ++i) o[i] = o[i] * f + v[i] * g;
-    m = top;
-  };
-  if (live) {
-    n = row % p.Nq;
-    head = row / p.Nq % p.Hq;
-    b = row / p.Nq / p.Hq;
-    const Line line = make_line(p, __ldcg(p.cum + p.B));
-    const int h = head / p.group, own = (head - h * p.group) * p.Nq + n;  // row among the sequence's
-    if (p.units_p > 0) {
-      const int stacked = b * p.rows_own + own;
-      const int u = h * p.blocks_p + stacked / X_ROWS, x = u * p.tiles_p * line.wp;
-      const int c0 = owner(line, x), c1 = owner(line, x + (p.tiles_p - 1) * line.wp);
-      for (int c = c0 + share; c <= c1; c += WARPS) add(static_cast<int64_t>(u + c) * X_ROWS + stacked % X_ROWS);
-    }
-    const int before = __ldcg(p.cum + b), tiles = __ldcg(p.cum + b + 1) - before;
-    if (tiles > 0) {
-      const int per_seq = p.Hkv * p.blocks_own, u = h * p.blocks_own + own / X_ROWS;
-      const int x = line.Wp + (before * per_seq + u * tiles) * line.ws;
-      const int c0 = owner(line, x), c1 = owner(line, x + (tiles - 1) * line.ws);
-      for (int c = c0 + share; c <= c1; c += WARPS)
-        add(static_cast<int64_t>(p.units_p + p.ctas) * X_ROWS + static_cast<int64_t>(b * per_seq + u + c) * p.own_slot + own % X_ROWS);
-    }
+    for (int i = 0; i < COLS; ++i) o[i] = fmaf(v.x[i], w, o[i]);
   }
-  if (WARPS > 1) {
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) part_o[warp][lane * COLS + i] = o[i];
-    if (lane == 0) part_m[warp] = m, part_l[warp] = l;
-    __syncthreads();
-    if (share) return;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part_m[warp + w]);
-    m = top, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) o[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float x = part_m[warp + w], f = x == -INFINITY ? 0.f : exp2f(x - top);
-      l += part_l[warp + w] * f;
-#pragma unroll
-      for (int i = 0; i < COLS; ++i) o[i] += part_o[warp + w][lane * COLS + i] * f;
-    }
-  }
-  if (!live) return;
-  const bool empty = l == 0.f;
-  const float inv = empty ? 0.f : 1.f / l;
+  const bool empty = total == 0.f;
+  const float inv = empty ? 0.f : 1.f / total;
+  const int head = h * p.group + own / p.Nq, n = own % p.Nq;
   __nv_bfloat16* dst = p.out + b * p.out_strides[0] + head * p.out_strides[1] + n * p.out_strides[2] + lane * COLS;
   if (COLS == 4)
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[COLS - 2] * inv, o[COLS - 1] * inv));
   else
     *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0] * inv, o[1] * inv);
   if (p.lse && lane == 0) {
-    const float x = empty ? INFINITY : m + log2f(l);
+    const float x = empty ? INFINITY : top + log2f(total);
     p.lse[b * p.lse_strides[0] + head * p.lse_strides[1] + n] = p.lse_natural ? x * 0.6931471805599453f : x;
   }
 }
 
+// How a call is divided.
 struct Sizes {
-  int rows_own, own_slot, blocks_own, blocks_p, units_p, tiles_p, tiles_own, ctas;
-  int64_t row_slots, cum_bytes, bytes;
+  int rows_own, blocks_p, units_p, tiles_p, cluster, splits;
+  int by_rows, blocks_own, own_slot, units_own, pieces;
+  int64_t own_parts, row_slots, cum_bytes, bytes;
 };
+
+// CTAs of a cluster and clusters of a unit.  A CTA is taken to cost a start and end (more in a larger cluster), and its
+// tiles, which go faster where it has an SM to itself; clusters of a unit beyond one cost the kernel that adds them up.
+void divide_prefix(int sms, Sizes& z) {
+  double best = 0;
+  for (int cluster = 1; cluster <= X_CLUSTER; cluster *= 2)
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      const int64_t shares = static_cast<int64_t>(cluster) * splits;
+      if (shares > 1 && (shares > z.tiles_p || (splits > 1 && cluster < 8))) continue;
+      const int64_t ctas = z.units_p * shares, waves = (ctas + 2 * sms - 1) / (2 * sms);
+      const double tiles = static_cast<double>((z.tiles_p + shares - 1) / shares);
+      const double cost = waves * (4.0 + 0.15 * cluster + tiles * (ctas <= sms ? 0.65 : 1.1)) + (splits > 1 ? 4.0 : 0.0);
+      if (shares == 1 || cost < best) best = cost, z.cluster = cluster, z.splits = splits;
+    }
+}
 
 // false if the problem is beyond the kernels' 32-bit counts.
 bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Sizes& z) {
   const int64_t rows_own = static_cast<int64_t>(Hq / Hkv) * Nq, rows_all = rows_own * B;
   if (rows_all * Hkv > INT32_MAX / 2) return false;
   z.rows_own = static_cast<int>(rows_own);
-  z.own_slot = rows_own < X_ROWS ? z.rows_own : X_ROWS;
-  z.blocks_own = static_cast<int>((rows_own + X_ROWS - 1) / X_ROWS);
   z.blocks_p = static_cast<int>((rows_all + X_ROWS - 1) / X_ROWS);
   z.tiles_p = P / X_KEYS + (P % X_KEYS != 0);
-  z.tiles_own = S / X_KEYS + (S % X_KEYS != 0);
   z.units_p = z.tiles_p ? Hkv * z.blocks_p : 0;
-  const int64_t units_own = static_cast<int64_t>(B) * Hkv * z.blocks_own;
-  const int64_t tiles = static_cast<int64_t>(z.units_p) * z.tiles_p + units_own * z.tiles_own;
-  if (tiles > INT32_MAX / 16) return false;
-  z.ctas = static_cast<int>(tiles < 2 * sms ? (tiles > 0 ? tiles : 1) : 2 * sms);
-  z.row_slots = static_cast<int64_t>(z.units_p + z.ctas) * X_ROWS + (units_own + z.ctas) * z.own_slot;
+  z.cluster = z.splits = 1;
+  if (z.units_p) divide_prefix(sms, z);
+  z.by_rows = rows_own <= Y_FEW_ROWS;
+  const int unit_rows = z.by_rows ? R_ROWS : X_ROWS;
+  z.own_slot = rows_own < unit_rows ? z.rows_own : unit_rows;
+  z.blocks_own = static_cast<int>((rows_own + unit_rows - 1) / unit_rows);
+  const int64_t units = S ? static_cast<int64_t>(B) * Hkv * z.blocks_own : 0, steps = units * ((S + 15ll) / 16 + Y_START);
+  if (steps > INT32_MAX / 16 || static_cast<int64_t>(z.units_p) * z.cluster * z.splits > INT32_MAX / 2) return false;
+  z.units_own = static_cast<int>(units);
+  // every warp of two CTAs per SM has a piece, but a unit no more than 32: whoever adds them goes through all of them
+  z.pieces = 0;
+  if (z.by_rows && S) {
+    const int64_t warps = 2ll * sms * Y_WARPS, most = steps < 32 * units ? steps : 32 * units;
+    z.pieces = static_cast<int>(most < warps ? most : warps);
+  }
+  z.own_parts = z.splits > 1 ? static_cast<int64_t>(z.units_p) * z.splits * X_ROWS : 0;
+  z.row_slots = z.own_parts + (units + z.pieces) * z.own_slot;
   z.cum_bytes = (static_cast<int64_t>(B) * 4 + 4 + 15) / 16 * 16;
-  z.bytes = z.cum_bytes + z.row_slots * (d + 2) * 4;
+  z.bytes = z.cum_bytes + z.row_slots * (d + 1) * 4;
   return true;
 }
 
 template <bool FP8, int DH>
-int launch_prefix(const CUtensorMap (&maps)[4], PrefixParams& p, cudaStream_t stream) {
+int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p, cudaStream_t stream) {
   using C = PrefixCfg<FP8, DH>;
   static_assert(2 * (C::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
-  const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH>);
-  if (allow_smem(fn, C::SMEM)) return WK_E_CUDA;
-  if (int bad = launch_pdl(fn, dim3(p.ctas), X_THREADS, C::SMEM, stream, 1,
-                           {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]),
-                            const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]), &p}))
-    return bad;
-  // few rows have many segments each: a CTA for a row
-  const int rows = p.B * p.Hq * p.Nq;
-  if (rows <= 8 * 148)
-    return launch_pdl(reinterpret_cast<const void*>(attn_prefix_combine_kernel<DH, 8>), dim3(rows), 256, 0, stream, 1, {&p});
-  return launch_pdl(reinterpret_cast<const void*>(attn_prefix_combine_kernel<DH, 1>), dim3((rows + 7) / 8), 256, 0, stream, 1,
-                    {&p});
+  if (z.units_own && z.by_rows) {
+    const void* fn = reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH>);
+    constexpr int ring = Y_WARPS * Y_STAGES * RowsCfg<FP8, DH>::STAGE_BYTES;
+    if (allow_smem(fn, ring)) return WK_E_CUDA;
+    if (int bad = launch_pdl(fn, dim3((z.pieces + Y_WARPS - 1) / Y_WARPS), 32 * Y_WARPS, ring, stream, 1, {&p})) return bad;
+  } else if (z.units_own) {
+    const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH, true>);
+    if (allow_smem(fn, C::SMEM)) return WK_E_CUDA;
+    if (int bad = launch_pdl(fn, dim3(z.units_own), X_THREADS, C::SMEM, stream, 1,
+                             {const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]), &p}))
+      return bad;
+  }
+  if (z.units_p) {
+    const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH, false>);
+    if (allow_smem(fn, C::SMEM) || allow_large_clusters(fn)) return WK_E_CUDA;
+    if (int bad = launch_pdl(fn, dim3(z.units_p * z.splits * z.cluster), X_THREADS, C::SMEM, stream, z.cluster,
+                             {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]), &p}))
+      return bad;
+    if (z.splits == 1) return 0;
+  }
+  return launch_pdl(reinterpret_cast<const void*>(attn_prefix_combine_kernel<DH>), dim3((p.Hkv * p.rows_all + 7) / 8), 256, 0,
+                    stream, 1, {&p});
 }
 
 }  // namespace
@@ -780,16 +1010,17 @@ extern "C" int wk_attn_fwd_shared_prefix(const wk_attn_prefix_args* a, void* str
   for (int i = 0; i < 3; ++i) p.q_strides[i] = a->q_strides[i] * size, p.out_strides[i] = a->out_strides[i];
   p.lse_strides[0] = a->lse_strides[0], p.lse_strides[1] = a->lse_strides[1];
   p.B = a->B, p.Hq = a->Hq, p.Hkv = a->Hkv, p.group = a->Hq / a->Hkv, p.Nq = a->Nq, p.P = a->P, p.S = a->S;
-  p.rows_own = z.rows_own, p.rows_all = z.rows_own * a->B, p.own_slot = z.own_slot;
-  p.units_p = z.units_p, p.blocks_p = z.blocks_p, p.blocks_own = z.blocks_own, p.tiles_p = z.tiles_p, p.ctas = z.ctas;
-  p.weight_p = 1, p.weight_own = 2;
+  p.rows_own = z.rows_own, p.rows_all = z.rows_own * a->B;
+  p.blocks_p = z.blocks_p, p.tiles_p = z.tiles_p, p.cluster = z.cluster, p.splits = z.splits;
+  p.by_rows = z.by_rows, p.blocks_own = z.blocks_own, p.own_slot = z.own_slot, p.pieces = z.pieces, p.own_parts = z.own_parts;
+  p.k = static_cast<const uint8_t*>(a->k), p.v = static_cast<const uint8_t*>(a->v);
+  for (int i = 0; i < 3; ++i) p.k_strides[i] = a->k_strides[i] * size, p.v_strides[i] = a->v_strides[i] * size;
   p.causal = a->causal, p.lse_natural = a->lse_natural;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.cum = static_cast<int*>(a->workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + z.cum_bytes);
   p.part_lse = p.part + z.row_slots * a->d;
-  p.part_top = p.part_lse + z.row_slots;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (fp8) return a->d == 64 ? launch_prefix<true, 64>(maps, p, st) : launch_prefix<true, 128>(maps, p, st);
-  return a->d == 64 ? launch_prefix<false, 64>(maps, p, st) : launch_prefix<false, 128>(maps, p, st);
+  if (fp8) return a->d == 64 ? launch_prefix<true, 64>(maps, z, p, st) : launch_prefix<true, 128>(maps, z, p, st);
+  return a->d == 64 ? launch_prefix<false, 64>(maps, z, p, st) : launch_prefix<false, 128>(maps, z, p, st);
 }

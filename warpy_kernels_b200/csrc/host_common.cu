@@ -113,30 +113,40 @@ int sm_count() {
   return g_sms[dev];
 }
 
-int allow_smem(const void* func, int bytes) {
-  // remembered per (kernel, device): the attribute belongs to the device's context
-  constexpr int kMaxFuncs = 64;
-  static const void* funcs[kMaxFuncs] = {};
+namespace {
+// Sets an attribute of a kernel once per (kernel, attribute, device): it belongs to the device's context.
+int set_once(const void* func, cudaFuncAttribute attribute, int value) {
+  constexpr int kMaxFuncs = 128;
+  static struct {
+    const void* func;
+    cudaFuncAttribute attribute;
+  } known[kMaxFuncs] = {};
   static bool done[kMaxFuncs][kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return WK_E_CUDA;
   std::lock_guard<std::mutex> lock(g_mu);
   int slot = -1;
   for (int i = 0; i < kMaxFuncs; ++i) {
-    if (funcs[i] == func || funcs[i] == nullptr) {
+    if ((known[i].func == func && known[i].attribute == attribute) || known[i].func == nullptr) {
       slot = i;
       break;
     }
   }
-  if (slot >= 0 && funcs[slot] == func && done[slot][dev]) return 0;
-  if (cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return WK_E_CUDA;
+  if (slot >= 0 && known[slot].func && done[slot][dev]) return 0;
+  if (cudaFuncSetAttribute(func, attribute, value) != cudaSuccess) return WK_E_CUDA;
   if (slot >= 0) {
-    funcs[slot] = func;
+    known[slot] = {func, attribute};
     done[slot][dev] = true;
   }
   return 0;
 }
+}  // namespace
+
+int allow_smem(const void* func, int bytes) {
+  return set_once(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+int allow_large_clusters(const void* func) { return set_once(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); }
 
 int clusters_at_once(const void* func, int size, int threads, int smem) {
   if (size == 1) return sm_count();  // every kernel that asks has one CTA per SM

@@ -33,6 +33,9 @@ int sm_count();
 // Raises the dynamic shared memory limit of `func` once per device.
 int allow_smem(const void* func, int bytes);
 
+// Lets `func` be launched in clusters of up to 16 CTAs, once per device.
+int allow_large_clusters(const void* func);
+
 // How many clusters of `size` CTAs of this kernel the current device runs at once (asked once per device).
 int clusters_at_once(const void* func, int size, int threads, int smem);
 
