@@ -8,8 +8,7 @@
 // times its queries) go over its own keys.
 //
 // Own keys come first, and leave parts: O / l and the log-sum-exp of every row, fp32.  Up to 32 rows a sequence, that is a
-// kernel on mma.sync whose warps work by themselves (bound by memory, and by latency where sequences are short); more
-// rows take the tensor-core kernel below, one CTA for 128 of them.
+// kernel on mma.sync whose warps work by themselves; more rows take the tensor-core kernel below, one CTA for 128 of them.
 // The prefix: a unit is 128 stacked rows, and S = Q.K^T and O += P.V go by 128 x 64 tiles on tcgen05.  A unit's tiles are
 // divided over the CTAs of a cluster, which meet in distributed shared memory, add the own keys' parts and write the output.
 // Where units are few, several clusters share one; then they leave parts too, and a last kernel adds up all of them.  The
@@ -22,13 +21,13 @@
 //
 // Numerics: logits in base 2.  Tensor-core kernel: the row reference is the maximum of the CTA's first tile (bf16 has the
 // exponent range to leave it there); a CTA in which a row rises more than 2^60 above it goes through its keys once more, with
-// the maxima it then knows.  Kernel for few rows: the moving reference of attn_rows.cu.
+// the maxima it then knows.  Kernel for few rows: the reference moves when a score exceeds it by more than 1; P is bf16, or
+// f16 times 2^14 for FP8 inputs, whose K and V become f16 (exact).
 #include <math.h>
 
 #include "common.cuh"
 #include "host_common.h"
 #include "pair.cuh"
-#include "rows16.cuh"
 #include "softmax16.cuh"
 
 namespace wk {
@@ -45,14 +44,14 @@ constexpr float X_MAX_EXP = 60.f;
 constexpr int X_CLUSTER = 16;  // largest cluster
 constexpr int X_PAD = 4;       // values between rows in the exchange: lanes with neighbouring rows write without conflicts
 
-constexpr int Y_STAGES = 3;
 constexpr int Y_START = 1;  // what a unit of the kernel for few rows weighs beside its steps
-constexpr int Y_WARPS = R_WARPS;
+constexpr int Y_WARPS = 4;
+constexpr int Y_ROWS = 16;      // rows of one of its units, at most
 constexpr int Y_FEW_ROWS = 32;  // rows of a sequence up to which that kernel takes them
 constexpr int Y_CUM = 1024;     // sequences whose weights are summed in shared memory
 
 struct PrefixParams {
-  const uint8_t *q, *k, *v;  // k, v: own keys and values
+  const uint8_t* q;
   const float* q_descale;
   const float* kp_descale;
   const float* vp_descale;
@@ -61,8 +60,8 @@ struct PrefixParams {
   const int* seqused;
   __nv_bfloat16* out;
   float* lse;
-  int64_t q_strides[3], k_strides[3], v_strides[3];  // bytes
-  int64_t out_strides[3], lse_strides[2];            // elements
+  int64_t q_strides[3];                    // bytes
+  int64_t out_strides[3], lse_strides[2];  // elements
   int B, Hq, Hkv, group, Nq, P, S;
   int rows_all;    // stacked rows of a KV head: B . group . Nq
   int rows_own;    // of one sequence
@@ -119,11 +118,11 @@ struct OwnParts {
     if (p.by_rows) {
       const int all = __ldcg(p.cum + p.B), before = __ldcg(p.cum + b), weight = __ldcg(p.cum + b + 1) - before;
       if (weight <= Y_START) return;
-      const int per_seq = p.Hkv * p.blocks_own, u = h * p.blocks_own + own / R_ROWS, x = before * per_seq + u * weight;
+      const int per_seq = p.Hkv * p.blocks_own, u = h * p.blocks_own + own / Y_ROWS, x = before * per_seq + u * weight;
       const Pieces line(all * per_seq, p.pieces);
       const int c = line.owner(x + Y_START);
       count = line.owner(x + weight - 1) - c + 1;
-      first = own_slot_of(p, b * per_seq + u, c) + own % R_ROWS;
+      first = own_slot_of(p, b * per_seq + u, c) + own % Y_ROWS;
     } else if (own_keys(p, b)) {
       count = 1;
       first = own_slot_of(p, (b * p.Hkv + h) * p.blocks_own + own / X_ROWS, 0) + own % X_ROWS;
@@ -165,6 +164,9 @@ struct PrefixCfg {
   static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowEnd)) <= X_AT, "");
 };
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -358,7 +360,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           asm volatile("ld.shared.b64 %0, [%1];" : "=l"(at) : "r"(smem + C::ROW_AT + row * 8) : "memory");
 #pragma unroll
           for (int span = 0; span < C::SPANS; ++span)
-            cp_async(smem + C::Q_AT + span * C::Q_SPAN + row * 128 + ((c ^ (row & 7)) << 4), p.q + at + span * 128 + 16 * c, 16);
+            cp_async16(smem + C::Q_AT + span * C::Q_SPAN + row * 128 + ((c ^ (row & 7)) << 4), p.q + at + span * 128 + 16 * c);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         fence_proxy_async_smem();
@@ -617,7 +619,17 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // ---- own keys of sequences with few rows ---------------------------------------------------------------------------
 // A unit is up to 16 rows of one (sequence, KV head) and its own keys, in steps of KEYS; it weighs one more than its steps,
 // for its start and end.  All units form a line that is cut into as many pieces as there are warps; a warp goes through its
-// piece by itself, its fetches three steps ahead and on into the next units, and leaves a part of every unit.
+// piece by itself, its loads running on into the next units, and leaves a part of every unit.
+//
+// Keys play the 16-row side of the MMAs and the rows the 8-column side, once or twice:
+//   S^T[16 keys, 8 rows] = K.Q^T     O^T[d, 8 rows] += V^T.P^T
+// so that a sequence's few rows leave little of an MMA empty and the accumulators take half the registers.  Tiles of K and V
+// come in turn by TMA into a ring of the warp's own (three times 4 KiB) and go to the MMAs by ldmatrix; P changes lanes with
+// movmatrix.  FP8: ldmatrix moves pairs of codes; which index of the head dimension a pair stands for is the same for K and
+// Q, and only moves O's rows for V.
+//
+// Bound by reading K and V once; with eight warps on an SM their latency is what shows.  About 110 instructions for 16
+// keys (FP8: 340 for 32).
 
 // Exclusive sums of the sequences' weights, by the whole CTA; `cum` is in shared or global memory.
 template <int KEYS>
@@ -645,6 +657,18 @@ __device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int
   if (b1 == p.B && b0 < p.B) cum[p.B] = at;
   __syncthreads();
 }
+
+template <bool FP8, int DH>
+struct OwnCfg {
+  static constexpr int SIZE = FP8 ? 1 : 2;
+  static constexpr int SPANS = DH * SIZE > 128 ? 2 : 1;  // 128-byte spans of a row (FP8, 64: the upper half is zeros)
+  static constexpr int KEYS = 32 / SPANS;                // of a step
+  static constexpr int SPAN_BYTES = KEYS * 128;
+  static constexpr int SLOT_BYTES = SPANS * SPAN_BYTES;  // 4 KiB
+  static constexpr int SLOTS = 3;
+  static constexpr int K16 = DH / 16;                    // MMAs over the head dimension
+  static constexpr float P_SHIFT = FP8 ? 14.f : 0.f;     // P is stored times 2^14
+};
 
 template <bool FP8, int DH>
 struct OwnWalker {
@@ -696,13 +720,60 @@ struct OwnWalker {
   }
 };
 
-template <bool FP8, int DH>
-__global__ void __launch_bounds__(32 * Y_WARPS, 2)
-attn_prefix_own_kernel(const __grid_constant__ PrefixParams p) {
-  using C = RowsCfg<FP8, DH>;
-  extern __shared__ __align__(16) uint8_t ring_mem[];
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if (F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) {
+  if (!F16) return pack_bf16x2(lo, hi);
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// NT: groups of eight rows, 1 or 2.
+template <bool FP8, int DH, int NT>
+__global__ void __launch_bounds__(32 * Y_WARPS, NT == 1 ? 4 : 3)
+attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ PrefixParams p) {
+  using C = OwnCfg<FP8, DH>;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ int cum_mem[Y_CUM + 1], warp_sums[Y_WARPS];
+  __shared__ __align__(8) uint64_t bar_mem[Y_WARPS][C::SLOTS];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * C::SLOTS * C::SLOT_BYTES;
+  const uint32_t bars = smem_u32(bar_mem[warp]);
+  if (lane == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) mbar_init(bars + 8 * i, 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
   pdl_wait();
   // the prefix kernel runs beside this one and reads what was written before it: it may start only now
   pdl_launch_dependents();
@@ -714,98 +785,241 @@ attn_prefix_own_kernel(const __grid_constant__ PrefixParams p) {
   const int blocks = p.blocks_own, per_seq = p.Hkv * blocks;
   const Pieces line(cum[p.B] * per_seq, p.pieces);
   const int piece = blockIdx.x * Y_WARPS + warp;
-  const uint32_t ring = smem_u32(ring_mem) + warp * Y_STAGES * C::STAGE_BYTES;
 
   OwnWalker<FP8, DH> now(p, line, cum, blocks, piece), ahead = now;
-  const uint8_t *k_base = nullptr, *v_base = nullptr;
-  auto start = [&]() {
-    k_base = p.k + ahead.b * p.k_strides[0] + ahead.h * p.k_strides[1] + t * 16;
-    v_base = p.v + ahead.b * p.v_strides[0] + ahead.h * p.v_strides[1] + g * C::V_PIECE;
-  };
-  auto fetch = [&](int stage) {
-    if (ahead.here()) {
-      const uint32_t ks = ring + stage * C::STAGE_BYTES + lane * 16;
-      const uint32_t vs = ring + stage * C::STAGE_BYTES + C::K_BYTES + lane * C::V_PIECE;
-      const int key0 = ahead.step * C::KEYS;
-#pragma unroll
-      for (int j = 0; j < C::N8; ++j) {  // keys beyond the last one are masked: any valid row will do
-        const uint8_t* src = k_base + min(key0 + 8 * j + g, ahead.nk - 1) * p.k_strides[2];
-#pragma unroll
-        for (int i = 0; i < C::K_PIECES; ++i) cp_async(ks + (j * C::K_PIECES + i) * 512, src + 64 * i, 16);
-      }
-#pragma unroll
-      for (int j = 0; j < C::KEYS / 4; ++j) {
-        const uint8_t* src = v_base + min(key0 + 8 * (j / 2) + 2 * t + (j & 1), ahead.nk - 1) * p.v_strides[2];
-#pragma unroll
-        for (int i = 0; i < C::V_PIECES; ++i)
-          cp_async(vs + (j * C::V_PIECES + i) * (32 * C::V_PIECE), src + 8 * C::V_PIECE * i, C::V_PIECE);
-      }
-      if (++ahead.step == ahead.end) {
-        ahead.next(p, cum, blocks);
-        if (ahead.here()) start();
-      }
+  // Slots are filled in turn: K of a step, V of it, K of the next.
+  int fetched = 0;
+  auto fetch = [&]() {
+    if (!ahead.here()) return;
+    const int slot = fetched % C::SLOTS, is_v = fetched & 1;
+    if (lane == 0) {
+      const uint32_t dst = ring + slot * C::SLOT_BYTES, bar = bars + 8 * slot;
+      mbar_expect_tx(bar, C::SLOT_BYTES);
+      for (int i = 0; i < C::SPANS; ++i)
+        tma_load_4d(dst + i * C::SPAN_BYTES, is_v ? &map_v : &map_k, bar, 64 * i, ahead.step * C::KEYS, ahead.h, ahead.b);
     }
-    cp_async_commit();
+    ++fetched;
+    if (is_v && ++ahead.step == ahead.end) ahead.next(p, cum, blocks);
   };
-  if (ahead.here()) start();
-  for (int i = 0; i < Y_STAGES; ++i) fetch(i);
+  for (int i = 0; i < C::SLOTS; ++i) fetch();
 
-  int stage = 0;
+  int used = 0;
+  bool ok = true;
+  auto arrive_at = [&]() {  // the slot in turn, its data there
+    const int slot = used % C::SLOTS;
+    ok = ok && mbar_wait_warp(bars + 8 * slot, (used / C::SLOTS) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
+    ++used;
+    return ring + slot * C::SLOT_BYTES;
+  };
   for (; now.here(); now.next(p, cum, blocks)) {
-    const int row0 = now.block * R_ROWS, sc = now.b * p.Hkv + now.h, unit = now.b * per_seq + now.u;
-    uint4 q[2][C::K_PIECES];
-    int limit[2], first_limit = now.nk - 1;  // last visible keys of the thread's two rows, and of all rows of the unit
+    const int row0 = now.block * Y_ROWS, sc = now.b * p.Hkv + now.h, unit = now.b * per_seq + now.u;
+    // Q: row g of each group of eight, the head dimension in the order of K's fragments
+    uint32_t q[NT][C::K16][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = min(row0 + g + 8 * i, p.rows_own - 1), n = r % p.Nq;
-      const uint8_t* src = p.q + now.b * p.q_strides[0] + (now.h * p.group + r / p.Nq) * p.q_strides[1] + n * p.q_strides[2] + t * 16;
+    for (int i = 0; i < NT; ++i) {
+      const int r = min(row0 + 8 * i + g, p.rows_own - 1);
+      const uint8_t* src = p.q + now.b * p.q_strides[0] + (now.h * p.group + r / p.Nq) * p.q_strides[1] + (r % p.Nq) * p.q_strides[2];
 #pragma unroll
-      for (int j = 0; j < C::K_PIECES; ++j) q[i][j] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * j));
-      limit[i] = p.causal ? min(now.nk - 1, n + now.nk - p.Nq) : now.nk - 1;
+      for (int k = 0; k < C::K16; ++k) {
+        if (FP8) {
+          const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(src + 16 * k + 4 * t));
+          q[i][k][0] = e4m3x2_to_f16x2(static_cast<uint16_t>(w)), q[i][k][1] = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+        } else {
+          q[i][k][0] = __ldcg(reinterpret_cast<const uint32_t*>(src + 32 * k + 4 * t));
+          q[i][k][1] = __ldcg(reinterpret_cast<const uint32_t*>(src + 32 * k + 16 + 4 * t));
+        }
+      }
     }
-    if (p.causal) first_limit = min(first_limit, now.nk - p.Nq);  // of query 0, whether it is among them or not
+    // this lane's rows in the accumulators are 2 t and 2 t + 1 of each group; the last keys they see
+    int limit[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = min(row0 + 8 * i + 2 * t + j, p.rows_own - 1);
+        limit[i][j] = p.causal ? min(now.nk - 1, r % p.Nq + now.nk - p.Nq) : now.nk - 1;
+      }
+    const int first_limit = p.causal ? min(now.nk - 1, now.nk - p.Nq) : now.nk - 1;  // of query 0, among them or not
     float beta = p.scale_log2, v_scale = 1.f;
     if (FP8) beta *= __ldcg(p.q_descale + sc) * __ldcg(p.k_descale + sc), v_scale = __ldcg(p.v_descale + sc);
 
-    float o[C::NT][4];
+    float o[NT][C::K16][4], m[NT][2], l[NT][2];
 #pragma unroll
-    for (int j = 0; j < C::NT; ++j)
+    for (int i = 0; i < NT; ++i) {
+      m[i][0] = m[i][1] = -INFINITY, l[i][0] = l[i][1] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int step = now.step; step < now.end; ++step) {
-      cp_async_wait<Y_STAGES - 1>();
-      rows_step<FP8, DH>(ring + stage * C::STAGE_BYTES + lane * 16,
-                         ring + stage * C::STAGE_BYTES + C::K_BYTES + lane * C::V_PIECE, q, beta, step * C::KEYS, first_limit,
-                         limit, t, o, m, l, top);
-      // the stage's own reads are done (their values have been used): refill it
-      fetch(stage);
-      if (++stage == Y_STAGES) stage = 0;
+      for (int k = 0; k < C::K16; ++k) o[i][k][0] = o[i][k][1] = o[i][k][2] = o[i][k][3] = 0.f;
     }
-
-    // ---- this warp's part: O / l and the log-sum-exp.  Column tile j of the MMAs holds element j % V_ELEMS of piece
-    // j / V_ELEMS of the eight lanes that share a V row.
-    const int64_t slot = own_slot_of(p, unit, piece);
+    for (int step = now.step; step < now.end; ++step) {
+      constexpr int N16 = C::KEYS / 16;
+      float s[NT][N16][4];  // keys g, g + 8 of each 16; rows 2 t, 2 t + 1
+      {
+        const uint32_t ks = arrive_at();
+        // ldmatrix: lane gives the row lane % 16 of 16 keys, 16-byte piece lane / 16 of two
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      const int r = g + 8 * i;
-      if (row0 + r < p.rows_own) {
-        const float inv = l[i] > 0.f ? v_scale / l[i] : l[i] == l[i] ? 0.f : l[i];
-        float* dst = p.part + (slot + r) * DH;
+        for (int n = 0; n < N16; ++n) {
 #pragma unroll
-        for (int j = 0; j < C::NT; j += 4) {
-          float* at = dst + (j / C::V_ELEMS) * (8 * C::V_ELEMS) + 2 * t * C::V_ELEMS + j % C::V_ELEMS;
-          *reinterpret_cast<float4*>(at) = make_float4(o[j][2 * i] * inv, o[j + 1][2 * i] * inv, o[j + 2][2 * i] * inv,
-                                                       o[j + 3][2 * i] * inv);
-          *reinterpret_cast<float4*>(at + C::V_ELEMS) = make_float4(
-              o[j][2 * i + 1] * inv, o[j + 1][2 * i + 1] * inv, o[j + 2][2 * i + 1] * inv, o[j + 3][2 * i + 1] * inv);
+          for (int i = 0; i < NT; ++i) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
+          const int key = 16 * n + lane % 16;
+          if (FP8) {
+#pragma unroll
+            for (int k = 0; k < C::K16; k += 2) {  // two pieces: 32 elements
+              uint32_t w[4], a[2][4];
+              ldmatrix_x4(w, ks + key * 128 + (((k + lane / 16) ^ (key & 7)) << 4));
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                a[x][0] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 * x])), a[x][2] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 * x] >> 16));
+                a[x][1] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 * x + 1]));
+                a[x][3] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 * x + 1] >> 16));
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+                  mma_16816<true>(s[i][n], a[x][0], a[x][1], a[x][2], a[x][3], q[i][k + x][0], q[i][k + x][1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < C::K16; ++k) {
+              uint32_t a[4];
+              const int c = 2 * k + lane / 16;
+              ldmatrix_x4(a, ks + (c >> 3) * C::SPAN_BYTES + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+#pragma unroll
+              for (int i = 0; i < NT; ++i) mma_16816<false>(s[i][n], a[0], a[1], a[2], a[3], q[i][k][0], q[i][k][1]);
+            }
+          }
         }
-        if (t == 0) p.part_lse[slot + r] = l[i] == 0.f ? -INFINITY : m[i] - C::P_SHIFT + log2f(l[i]);
       }
       __syncwarp();
+      fetch();  // into K's place
+
+      const int key0 = step * C::KEYS;
+      const bool masked = key0 + C::KEYS - 1 > first_limit;
+      float mx[NT][2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int n = 0; n < N16; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][n][j] *= beta;
+            if (masked && key0 + 16 * n + g + 8 * (j >> 1) > limit[i][j & 1]) s[i][n][j] = -INFINITY;
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mx[i][j] = fmaxf(s[i][0][j], s[i][0][2 + j]);
+#pragma unroll
+          for (int n = 1; n < N16; ++n) mx[i][j] = max3(mx[i][j], s[i][n][j], s[i][n][2 + j]);
+        }
+      }
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mx[i][j] = fmaxf(mx[i][j], __shfl_xor_sync(0xffffffffu, mx[i][j], x));
+      bool move = false;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) move |= mx[i][0] > m[i][0] + 1.f || mx[i][1] > m[i][1] + 1.f;
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float f[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float to = mx[i][j] > m[i][j] + 1.f ? mx[i][j] : m[i][j];
+            f[j] = to > m[i][j] ? ex2_approx(m[i][j] - to) : 1.f;
+            m[i][j] = to;
+            l[i][j] *= f[j];
+          }
+#pragma unroll
+          for (int k = 0; k < C::K16; ++k) o[i][k][0] *= f[0], o[i][k][1] *= f[1], o[i][k][2] *= f[0], o[i][k][3] *= f[1];
+        }
+      }
+      uint32_t pt[NT][N16][2];  // P^T: row g, keys 2 t and 2 t + 1 of each eight
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float bias[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) bias[j] = m[i][j] > -INFINITY ? C::P_SHIFT - m[i][j] : 0.f;
+#pragma unroll
+        for (int n = 0; n < N16; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][n][j] = ex2_approx(s[i][n][j] + bias[j & 1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            l[i][j] += s[i][n][j] + s[i][n][2 + j];
+            pt[i][n][j] = movmatrix(pack_16x2<FP8>(s[i][n][2 * j], s[i][n][2 * j + 1]));
+          }
+        }
+      }
+
+      const uint32_t vs = arrive_at();
+      if (key0 + C::KEYS > now.nk) {
+        // rows of V behind the last key: whatever the cache holds there, 0 . V has to be 0
+        for (int x = lane; x < C::KEYS * C::SPANS * 8; x += 32) {
+          const int key = x / 8 % C::KEYS;
+          if (key0 + key >= now.nk) sts128(vs + x * 16, 0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();  // before TMA writes there again
+        __syncwarp();
+      }
+      // ldmatrix, transposed: matrices (keys 0-7, piece 0), (0-7, 1), (8-15, 0), (8-15, 1)
+#pragma unroll
+      for (int n = 0; n < N16; ++n) {
+        const int key = 16 * n + lane % 8 + lane / 16 * 8;
+        if (FP8) {
+#pragma unroll
+          for (int k = 0; k < C::K16; k += 2) {
+            uint32_t w[4];
+            ldmatrix_x4_trans(w, vs + key * 128 + (((k + lane / 8 % 2) ^ (key & 7)) << 4));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // 16 elements: pair g of the codes becomes rows g and g + 8
+              const uint32_t y0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x])), y1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x] >> 16));
+              const uint32_t z0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 + x])), z1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 + x] >> 16));
+              const uint32_t a0 = __byte_perm(y0, y1, 0x5410), a1 = __byte_perm(y0, y1, 0x7632);
+              const uint32_t a2 = __byte_perm(z0, z1, 0x5410), a3 = __byte_perm(z0, z1, 0x7632);
+#pragma unroll
+              for (int i = 0; i < NT; ++i) mma_16816<true>(o[i][k + x], a0, a1, a2, a3, pt[i][n][0], pt[i][n][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < C::K16; ++k) {
+            uint32_t a[4];
+            const int c = 2 * k + lane / 8 % 2;
+            ldmatrix_x4_trans(a, vs + (c >> 3) * C::SPAN_BYTES + key * 128 + (((c & 7) ^ (key & 7)) << 4));
+#pragma unroll
+            for (int i = 0; i < NT; ++i) mma_16816<false>(o[i][k], a[0], a[1], a[2], a[3], pt[i][n][0], pt[i][n][1]);
+          }
+        }
+      }
+      __syncwarp();
+      fetch();  // into V's place
     }
+
+    // ---- this warp's part: O / l and the log-sum-exp
+    const int64_t slot = own_slot_of(p, unit, piece);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], x);
+        const int r = 8 * i + 2 * t + j;
+        if (row0 + r < p.rows_own) {
+          const float inv = l[i][j] > 0.f ? v_scale / l[i][j] : l[i][j] == l[i][j] ? 0.f : l[i][j];
+          float* dst = p.part + (slot + r) * DH;
+#pragma unroll
+          for (int k = 0; k < C::K16; ++k)
+            if (FP8) {
+              *reinterpret_cast<float2*>(dst + 16 * k + 2 * g) = make_float2(o[i][k][j] * inv, o[i][k][2 + j] * inv);
+            } else {
+              dst[16 * k + g] = o[i][k][j] * inv;
+              dst[16 * k + g + 8] = o[i][k][2 + j] * inv;
+            }
+          if (g == 0) p.part_lse[slot + r] = l[i][j] == 0.f ? -INFINITY : m[i][j] - C::P_SHIFT + log2f(l[i][j]);
+        }
+        __syncwarp();
+      }
   }
 }
 
@@ -896,7 +1110,7 @@ bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Size
   z.cluster = z.splits = 1;
   if (z.units_p) divide_prefix(sms, z);
   z.by_rows = rows_own <= Y_FEW_ROWS;
-  const int unit_rows = z.by_rows ? R_ROWS : X_ROWS;
+  const int unit_rows = z.by_rows ? Y_ROWS : X_ROWS;
   z.own_slot = rows_own < unit_rows ? z.rows_own : unit_rows;
   z.blocks_own = static_cast<int>((rows_own + unit_rows - 1) / unit_rows);
   const int64_t units = S ? static_cast<int64_t>(B) * Hkv * z.blocks_own : 0, steps = units * ((S + 15ll) / 16 + Y_START);
@@ -920,10 +1134,14 @@ int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p,
   using C = PrefixCfg<FP8, DH>;
   static_assert(2 * (C::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
   if (z.units_own && z.by_rows) {
-    const void* fn = reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH>);
-    constexpr int ring = Y_WARPS * Y_STAGES * RowsCfg<FP8, DH>::STAGE_BYTES;
+    using Own = OwnCfg<FP8, DH>;
+    const void* fn = z.own_slot <= 8 ? reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 1>)
+                                     : reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 2>);
+    constexpr int ring = Y_WARPS * Own::SLOTS * Own::SLOT_BYTES + 1024;
     if (allow_smem(fn, ring)) return WK_E_CUDA;
-    if (int bad = launch_pdl(fn, dim3((z.pieces + Y_WARPS - 1) / Y_WARPS), 32 * Y_WARPS, ring, stream, 1, {&p})) return bad;
+    if (int bad = launch_pdl(fn, dim3((z.pieces + Y_WARPS - 1) / Y_WARPS), 32 * Y_WARPS, ring, stream, 1,
+                             {const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]), &p}))
+      return bad;
   } else if (z.units_own) {
     const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH, true>);
     if (allow_smem(fn, C::SMEM)) return WK_E_CUDA;
@@ -989,9 +1207,10 @@ extern "C" int wk_attn_fwd_shared_prefix(const wk_attn_prefix_args* a, void* str
   CUtensorMap maps[4] = {};
   const void* bases[4] = {a->k_prefix, a->v_prefix, a->k, a->v};
   const int64_t* strides[4] = {a->k_prefix_strides, a->v_prefix_strides, a->k_strides, a->v_strides};
-  const uint32_t box[4] = {fp8 ? 128u : 64u, X_KEYS, 1, 1};
   for (int i = 0; i < 4; ++i) {
     const int len = i < 2 ? a->P : a->S;
+    // own keys of few rows come in steps of 4 KiB, 128 bytes of a row at a time
+    const uint32_t box[4] = {fp8 ? 128u : 64u, i < 2 || !z.by_rows ? X_KEYS : !fp8 && a->d == 128 ? 16u : 32u, 1, 1};
     if (!len) continue;  // no tile of it is ever loaded
     const uint64_t dims[4] = {static_cast<uint64_t>(a->d), static_cast<uint64_t>(len), static_cast<uint64_t>(a->Hkv),
                               static_cast<uint64_t>(i < 2 ? 1 : a->B)};
@@ -1013,8 +1232,6 @@ extern "C" int wk_attn_fwd_shared_prefix(const wk_attn_prefix_args* a, void* str
   p.rows_own = z.rows_own, p.rows_all = z.rows_own * a->B;
   p.blocks_p = z.blocks_p, p.tiles_p = z.tiles_p, p.cluster = z.cluster, p.splits = z.splits;
   p.by_rows = z.by_rows, p.blocks_own = z.blocks_own, p.own_slot = z.own_slot, p.pieces = z.pieces, p.own_parts = z.own_parts;
-  p.k = static_cast<const uint8_t*>(a->k), p.v = static_cast<const uint8_t*>(a->v);
-  for (int i = 0; i < 3; ++i) p.k_strides[i] = a->k_strides[i] * size, p.v_strides[i] = a->v_strides[i] * size;
   p.causal = a->causal, p.lse_natural = a->lse_natural;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.cum = static_cast<int*>(a->workspace);
