@@ -49,6 +49,7 @@ constexpr int Y_WARPS = 4;
 constexpr int Y_ROWS = 16;      // rows of one of its units, at most
 constexpr int Y_FEW_ROWS = 32;  // rows of a sequence up to which that kernel takes them
 constexpr int Y_CUM = 1024;     // sequences whose weights are summed in shared memory
+constexpr int OWN_PARTS = 32;   // parts of a unit of own keys, at most
 
 struct PrefixParams {
   const uint8_t* q;
@@ -72,10 +73,12 @@ struct PrefixParams {
   int by_rows;     // own keys go to the kernel for few rows
   int blocks_own;  // units of a sequence's rows: 16 rows each, or 128
   int own_slot;    // rows of one of their parts
-  int pieces;      // by_rows: pieces that the line of units may be cut into
+  int pieces;      // by_rows: pieces that the line of units may be cut into,
+  int least;       // and how long they are at least: no unit then has more than OWN_PARTS parts
   int causal, lse_natural;
   float scale_log2;  // softmax_scale . log2(e)
   int* cum;          // [B + 1] by_rows: weight of the sequences' units before each of them
+  int* lengths;      // [B] by_rows: own keys of the sequences
   float* part;       // O / l of row slots [DH]: the prefix's, 128 a unit and split, then those of own keys
   float* part_lse;   // [row slot]
   int64_t own_parts;  // first row slot of own keys
@@ -91,9 +94,9 @@ __device__ __forceinline__ int own_keys(const PrefixParams& p, int b) {
 struct Pieces {
   int W, G;
   int size, longer;  // of a piece; how many (the first ones) are one longer
-  __device__ __forceinline__ Pieces(int weight, int most) {
-    W = weight, G = min(weight, most);
-    size = G ? W / G : 0;
+  __device__ __forceinline__ Pieces(int weight, int most, int least) {
+    W = weight, G = max(min(most, W / least), 1);
+    size = W / G;
     longer = W - size * G;
   }
   __device__ __forceinline__ int start(int c) const { return c * size + min(c, longer); }
@@ -119,7 +122,7 @@ struct OwnParts {
       const int all = __ldcg(p.cum + p.B), before = __ldcg(p.cum + b), weight = __ldcg(p.cum + b + 1) - before;
       if (weight <= Y_START) return;
       const int per_seq = p.Hkv * p.blocks_own, u = h * p.blocks_own + own / Y_ROWS, x = before * per_seq + u * weight;
-      const Pieces line(all * per_seq, p.pieces);
+      const Pieces line(all * per_seq, p.pieces, p.least);
       const int c = line.owner(x + Y_START);
       count = line.owner(x + weight - 1) - c + 1;
       first = own_slot_of(p, b * per_seq + u, c) + own % Y_ROWS;
@@ -130,13 +133,18 @@ struct OwnParts {
   }
 };
 
-// How a row of the tensor-core kernel ends.
-struct RowEnd {
-  float weight[X_CLUSTER];  // of the members' parts
-  float top, inv;           // reference of all weights, 1 / their sum
-  int64_t first;            // own keys' parts, to be weighted with 2^(lse - top)
-  int64_t to;               // offset in the output, or row slot
+// How a row of the tensor-core kernel ends: where it goes and which parts own keys have left of it, found by the producer
+// warp while the last tiles are worked on; and what all its parts count.
+struct RowTarget {
+  int64_t first;    // row slot of the first part of own keys
+  int64_t to;       // offset in the output, or row slot
+  int64_t lse_to;
   int parts;
+};
+struct RowWeights {
+  float own[OWN_PARTS];     // of the parts of own keys
+  float member[X_CLUSTER];  // and of the cluster's
+  float inv;                // 1 / their sum
 };
 
 template <bool FP8, int DH>
@@ -157,11 +165,12 @@ struct PrefixCfg {
   // row reference, then l and largest score of each group; at the end the log-sum-exp of each row
   static constexpr int X_AT = V16_AT + (FP8 ? 2 * V16_BYTES : 0);
   static constexpr int ROW_AT = X_AT + 5 * X_ROWS * 4;  // where each row of Q is
-  static constexpr int BAR_AT = ROW_AT + X_ROWS * 8;
+  static constexpr int TARGET_AT = ROW_AT + X_ROWS * 8;
+  static constexpr int BAR_AT = TARGET_AT + X_ROWS * static_cast<int>(sizeof(RowTarget));
   static constexpr int SMEM = BAR_AT + 8 * (4 * STAGES + 8) + 16 + 1024;
   // the exchange of a cluster takes the place of the tiles
   static constexpr int PART_BYTES = X_ROWS * (DH + X_PAD) * 4;
-  static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowEnd)) <= X_AT, "");
+  static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowWeights)) <= X_AT, "");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -264,6 +273,34 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     tile0 = 0, tiles = (keys + X_KEYS - 1) / X_KEYS;
   }
 
+  const int rank = OWN ? 0 : blockIdx.x % p.cluster, members = OWN ? 1 : p.cluster;
+  const int mine = rank < rows ? (rows - rank + members - 1) / members : 0;  // the rows congruent to this CTA's rank
+  const bool final = !OWN && p.splits == 1;
+  uint8_t* smem_ptr = smem_raw + (smem - smem_u32(smem_raw));
+  RowTarget* targets = reinterpret_cast<RowTarget*>(smem_ptr + C::TARGET_AT);
+  auto find_targets = [&]() {  // by the producer warp
+    if (beside) pdl_wait();    // the parts of own keys are there
+    for (int i = lane; i < mine; i += 32) {
+      const int r = i * members + rank;
+      RowTarget e = {};
+      int seq = b, own = row0 + r;
+      if (!OWN) seq = own / p.rows_own, own -= seq * p.rows_own;
+      if (final) {
+        const int g = own / p.Nq, n = own - g * p.Nq, head = h * p.group + g;
+        e.to = seq * p.out_strides[0] + head * p.out_strides[1] + n * p.out_strides[2];
+        e.lse_to = seq * p.lse_strides[0] + head * p.lse_strides[1] + n;
+        if (beside) {
+          const OwnParts parts(p, seq, h, own);
+          e.first = parts.first, e.parts = parts.count;
+        }
+      } else {
+        e.to = OWN ? own_slot_of(p, blockIdx.x, 0) + r : static_cast<int64_t>(blockIdx.x / p.cluster) * X_ROWS + r;
+      }
+      targets[i] = e;
+    }
+  };
+  if (tiles == 0 && warp == 0) find_targets();
+
   bool ok = true;  // no wait of this thread's role has given up
   float lse_row = -INFINITY, inv_row = 0.f;  // softmax threads: of their row, what its O is multiplied with
   float m_ref = -INFINITY;
@@ -290,6 +327,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
       __syncwarp();
+      if (pass == 0) find_targets();
     } else if (warp == 1) {
       const bool mine = elect_one();
       constexpr uint32_t idesc_qk = FP8 ? make_idesc(0, 0, 0, 0, X_ROWS, X_KEYS) : make_idesc(1, 1, 0, 0, X_ROWS, X_KEYS);
@@ -496,7 +534,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   }
 
   // ---- this CTA's part to shared memory: every tile and product has been used
-  uint8_t* part = smem_raw + (smem - smem_u32(smem_raw));  // [row][DH + X_PAD]
+  uint8_t* part = smem_ptr;  // [row][DH + X_PAD]
   if (warp >= 2) {
     const int quad = warp & 3, grp = (warp - 2) >> 2, r = quad * 32 + lane;
     const uint32_t o_tmem = tmem + (static_cast<uint32_t>(quad * 32) << 16) + X_O_COL + grp * (DH / 2);
@@ -528,70 +566,66 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     tc_fence_after();
     tmem_dealloc(tmem, X_TMEM_COLS);
   }
-  const bool final = !OWN && p.splits == 1;
-  if (beside) pdl_wait();  // the parts of own keys are there, and nothing that comes after this kernel starts before them
 
-  // ---- the rows congruent to this CTA's rank: first what each member's part and the own keys' parts count, one thread to
-  // a row, then the sums, a warp or half of one to a row
-  const int rank = OWN ? 0 : blockIdx.x % p.cluster, members = OWN ? 1 : p.cluster;
-  const int mine = rank < rows ? (rows - rank + members - 1) / members : 0;
-  RowEnd* ends = reinterpret_cast<RowEnd*>(part + C::PART_BYTES);
-  for (int i = threadIdx.x; i < mine; i += X_THREADS) {
-    const int r = i * members + rank;
-    const uint32_t stat = smem + C::X_AT + r * 4;
-    RowEnd e;
-    float top = -INFINITY, total = 0.f;
+  // ---- this CTA's rows: what each of their parts counts, one thread to a row, then the sums
+  if (beside) pdl_wait();  // nothing that comes after this kernel starts before the one for own keys has ended
+  RowWeights* weights = reinterpret_cast<RowWeights*>(part + C::PART_BYTES);
+  if (final && beside) {
+    for (int i = threadIdx.x; i < mine * OWN_PARTS; i += X_THREADS) {
+      const RowTarget& e = targets[i / OWN_PARTS];
+      const int k = i % OWN_PARTS;
+      if (k < e.parts) weights[i / OWN_PARTS].own[k] = __ldcg(p.part_lse + e.first + k * p.own_slot);
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < mine) {
+    const RowTarget& at = targets[threadIdx.x];
+    RowWeights& e = weights[threadIdx.x];
+    const uint32_t stat = smem + C::X_AT + (threadIdx.x * members + rank) * 4;
+    float lse[X_CLUSTER], top = -INFINITY, total = 0.f;
 #pragma unroll
     for (int k = 0; k < X_CLUSTER; ++k) {
-      e.weight[k] = -INFINITY;
-      if (k < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(e.weight[k]) : "r"(meet ? mapa(stat, k) : stat));
+      lse[k] = -INFINITY;
+      if (k < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(lse[k]) : "r"(meet ? mapa(stat, k) : stat));
     }
 #pragma unroll
-    for (int k = 0; k < X_CLUSTER; ++k) top = fmaxf(top, e.weight[k]);
-    int seq = b, own = row0 + r;
-    if (!OWN) seq = own / p.rows_own, own -= seq * p.rows_own;
-    e.parts = 0;
-    if (final && p.S) {
-      const OwnParts parts(p, seq, h, own);
-      e.first = parts.first, e.parts = parts.count;
-      for (int k = 0; k < parts.count; ++k) top = fmaxf(top, __ldcg(p.part_lse + parts.first + k * parts.distance));
-      for (int k = 0; k < parts.count; ++k) {
-        const float lse = __ldcg(p.part_lse + parts.first + k * parts.distance);
-        total += lse == -INFINITY ? 0.f : exp2f(lse - top);
-      }
+    for (int k = 0; k < X_CLUSTER; ++k) top = fmaxf(top, lse[k]);
+    for (int k = 0; k < at.parts; ++k) top = fmaxf(top, e.own[k]);
+    for (int k = 0; k < at.parts; ++k) {
+      e.own[k] = e.own[k] == -INFINITY ? 0.f : exp2f(e.own[k] - top);
+      total += e.own[k];
     }
 #pragma unroll
     for (int k = 0; k < X_CLUSTER; ++k) {
-      e.weight[k] = e.weight[k] == -INFINITY ? 0.f : exp2f(e.weight[k] - top);
-      total += e.weight[k];
+      e.member[k] = lse[k] == -INFINITY ? 0.f : exp2f(lse[k] - top);
+      total += e.member[k];
     }
     const bool empty = total == 0.f;
-    e.top = top, e.inv = empty ? 0.f : 1.f / total;
-    const float lse = empty ? INFINITY : top + log2f(total);
-    if (final) {
-      const int g = own / p.Nq, n = own - g * p.Nq, head = h * p.group + g;
-      e.to = seq * p.out_strides[0] + head * p.out_strides[1] + n * p.out_strides[2];
-      if (p.lse) p.lse[seq * p.lse_strides[0] + head * p.lse_strides[1] + n] = p.lse_natural ? lse * 0.6931471805599453f : lse;
-    } else {
-      e.to = OWN ? own_slot_of(p, blockIdx.x, 0) + r : static_cast<int64_t>(blockIdx.x / p.cluster) * X_ROWS + r;
-      p.part_lse[e.to] = empty ? -INFINITY : lse;
-    }
-    ends[i] = e;
+    e.inv = empty ? 0.f : 1.f / total;
+    const float y = empty ? INFINITY : top + log2f(total);
+    if (!final) p.part_lse[at.to] = empty ? -INFINITY : y;
+    else if (p.lse) p.lse[at.lse_to] = p.lse_natural ? y * 0.6931471805599453f : y;
   }
   __syncthreads();
   constexpr int QUADS = DH / 4;
   for (int i = threadIdx.x; i < mine * QUADS; i += X_THREADS) {
     const int c = i % QUADS, r = i / QUADS * members + rank;
-    const RowEnd& e = ends[i / QUADS];
+    const RowTarget& e = targets[i / QUADS];
+    const RowWeights& w = weights[i / QUADS];
     const uint32_t at = smem + r * (DH + X_PAD) * 4 + c * 16;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float w, const float4& v) {
-      o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+    auto add = [&](float f, const float4& v) {
+      o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
     };
-    for (int k = 0; k < e.parts; ++k) {
-      const int64_t slot = e.first + k * p.own_slot;
-      const float lse = __ldcg(p.part_lse + slot);
-      add(lse == -INFINITY ? 0.f : exp2f(lse - e.top), __ldcg(reinterpret_cast<const float4*>(p.part + slot * DH) + c));
+    for (int k0 = 0; k0 < e.parts; k0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < e.parts) v[k] = __ldcg(reinterpret_cast<const float4*>(p.part + (e.first + (k0 + k) * p.own_slot) * DH) + c);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) add(k0 + k < e.parts ? w.own[k0 + k] : 0.f, v[k]);
     }
     for (int k0 = 0; k0 < members; k0 += 8) {
       float4 v[8];
@@ -604,9 +638,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                        : "r"(meet ? mapa(at, k0 + k) : at));
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) add(e.weight[k0 + k], v[k]);
+      for (int k = 0; k < 8; ++k) add(w.member[k0 + k], v[k]);
     }
-    o.x *= e.inv, o.y *= e.inv, o.z *= e.inv, o.w *= e.inv;
+    o.x *= w.inv, o.y *= w.inv, o.z *= w.inv, o.w *= w.inv;
     if (final)
       *reinterpret_cast<uint2*>(p.out + e.to + 4 * c) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
     else
@@ -631,14 +665,18 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // Bound by reading K and V once; with eight warps on an SM their latency is what shows.  About 110 instructions for 16
 // keys (FP8: 340 for 32).
 
-// Exclusive sums of the sequences' weights, by the whole CTA; `cum` is in shared or global memory.
+// Exclusive sums of the sequences' weights, by the whole CTA, and their lengths; both in shared or global memory.
 template <int KEYS>
-__device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int* warp_sums) {
+__device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int* lengths, int* warp_sums) {
   constexpr int THREADS = 32 * Y_WARPS;
   const int per = (p.B + THREADS - 1) / THREADS, b0 = threadIdx.x * per, b1 = min(p.B, b0 + per);
-  auto weight = [&](int b) { return (own_keys(p, b) + KEYS - 1) / KEYS + Y_START; };
+  auto weight = [](int n) { return (n + KEYS - 1) / KEYS + Y_START; };
   int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += weight(b);
+  for (int b = b0; b < b1; ++b) {
+    const int n = own_keys(p, b);
+    lengths[b] = n;
+    sum += weight(n);
+  }
   int scan = sum;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
@@ -652,7 +690,7 @@ __device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int
   for (int w = 0; w < warp; ++w) at += warp_sums[w];
   for (int b = b0; b < b1; ++b) {
     cum[b] = at;
-    at += weight(b);
+    at += weight(lengths[b]);
   }
   if (b1 == p.B && b0 < p.B) cum[p.B] = at;
   __syncthreads();
@@ -675,9 +713,11 @@ struct OwnWalker {
   int x, x1;           // where in the line, end of the piece
   int b, h, block, u;  // sequence, KV head, 16 rows; u = h . blocks + block
   int weight, nk, step, end, base;
-  __device__ __forceinline__ void open(const PrefixParams& p, const int* cum) {
+  const int* cum;
+  const int* lengths;
+  __device__ __forceinline__ void open() {
     weight = cum[b + 1] - cum[b];
-    nk = own_keys(p, b);
+    nk = lengths[b];
   }
   // Steps of the piece in the unit that starts at `at`.
   __device__ __forceinline__ void range(int at) {
@@ -685,7 +725,9 @@ struct OwnWalker {
     step = max(0, x - base - Y_START);
     end = min(weight, x1 - base) - Y_START;
   }
-  __device__ __forceinline__ OwnWalker(const PrefixParams& p, const Pieces& l, const int* cum, int blocks, int piece) {
+  __device__ __forceinline__ OwnWalker(const PrefixParams& p, const Pieces& l, const int* cum, const int* lengths, int blocks,
+                                       int piece)
+      : cum(cum), lengths(lengths) {
     x = x1 = 0;
     if (piece >= l.G) return;
     x = l.start(piece), x1 = l.start(piece + 1);
@@ -696,16 +738,16 @@ struct OwnWalker {
       if (cum[mid] * per_seq <= x) lo = mid; else hi = mid - 1;
     }
     b = lo;
-    open(p, cum);
+    open();
     const int first = cum[b] * per_seq;
     u = (x - first) / weight;
     h = u / blocks, block = u - h * blocks;
     range(first + u * weight);
-    if (step >= end) next(p, cum, blocks);
+    if (step >= end) next(p, blocks);
   }
   __device__ __forceinline__ bool here() const { return x < x1; }
   // To the next unit that this piece has part in.
-  __device__ __forceinline__ void next(const PrefixParams& p, const int* cum, int blocks) {
+  __device__ __forceinline__ void next(const PrefixParams& p, int blocks) {
     do {
       x = base + weight;  // where the next unit starts
       if (x >= x1) return;
@@ -713,7 +755,7 @@ struct OwnWalker {
       if (++block == blocks) block = 0, ++h;
       if (u == p.Hkv * blocks) {
         u = h = 0, ++b;
-        open(p, cum);
+        open();
       }
       range(x);
     } while (step >= end);  // nothing of the unit but its start is in the piece, or it has no keys
@@ -759,12 +801,12 @@ __device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) {
 
 // NT: groups of eight rows, 1 or 2.
 template <bool FP8, int DH, int NT>
-__global__ void __launch_bounds__(32 * Y_WARPS, NT == 1 ? 4 : 3)
+__global__ void __launch_bounds__(32 * Y_WARPS) __maxnreg__(NT == 1 ? 112 : 168)
 attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ PrefixParams p) {
   using C = OwnCfg<FP8, DH>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int cum_mem[Y_CUM + 1], warp_sums[Y_WARPS];
+  __shared__ int cum_mem[Y_CUM + 1], length_mem[Y_CUM], warp_sums[Y_WARPS];
   __shared__ __align__(8) uint64_t bar_mem[Y_WARPS][C::SLOTS];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * C::SLOTS * C::SLOT_BYTES;
@@ -772,6 +814,8 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   if (lane == 0) {
     for (int i = 0; i < C::SLOTS; ++i) mbar_init(bars + 8 * i, 1);
     mbar_fence_init();
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
   }
   __syncwarp();
   pdl_wait();
@@ -779,29 +823,30 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   pdl_launch_dependents();
   // every CTA writes the same counts where they do not fit shared memory; those that add the parts read them from there
   int* cum = p.B <= Y_CUM ? cum_mem : p.cum;
-  sum_weights<C::KEYS>(p, cum, warp_sums);
+  int* lengths = p.B <= Y_CUM ? length_mem : p.lengths;
+  sum_weights<C::KEYS>(p, cum, lengths, warp_sums);
   if (blockIdx.x == 0 && cum != p.cum)
     for (int i = threadIdx.x; i <= p.B; i += 32 * Y_WARPS) p.cum[i] = cum[i];
   const int blocks = p.blocks_own, per_seq = p.Hkv * blocks;
-  const Pieces line(cum[p.B] * per_seq, p.pieces);
+  const Pieces line(cum[p.B] * per_seq, p.pieces, p.least);
   const int piece = blockIdx.x * Y_WARPS + warp;
 
-  OwnWalker<FP8, DH> now(p, line, cum, blocks, piece), ahead = now;
+  OwnWalker<FP8, DH> now(p, line, cum, lengths, blocks, piece), ahead = now;
   // Slots are filled in turn: K of a step, V of it, K of the next.
   int fetched = 0;
-  auto fetch = [&]() {
+  auto fetch = [&](int by) {
     if (!ahead.here()) return;
     const int slot = fetched % C::SLOTS, is_v = fetched & 1;
-    if (lane == 0) {
+    if (lane == by) {
       const uint32_t dst = ring + slot * C::SLOT_BYTES, bar = bars + 8 * slot;
       mbar_expect_tx(bar, C::SLOT_BYTES);
       for (int i = 0; i < C::SPANS; ++i)
         tma_load_4d(dst + i * C::SPAN_BYTES, is_v ? &map_v : &map_k, bar, 64 * i, ahead.step * C::KEYS, ahead.h, ahead.b);
     }
     ++fetched;
-    if (is_v && ++ahead.step == ahead.end) ahead.next(p, cum, blocks);
+    if (is_v && ++ahead.step == ahead.end) ahead.next(p, blocks);
   };
-  for (int i = 0; i < C::SLOTS; ++i) fetch();
+  for (int i = 0; i < C::SLOTS; ++i) fetch(0);
 
   int used = 0;
   bool ok = true;
@@ -811,7 +856,7 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     ++used;
     return ring + slot * C::SLOT_BYTES;
   };
-  for (; now.here(); now.next(p, cum, blocks)) {
+  for (; now.here(); now.next(p, blocks)) {
     const int row0 = now.block * Y_ROWS, sc = now.b * p.Hkv + now.h, unit = now.b * per_seq + now.u;
     // Q: row g of each group of eight, the head dimension in the order of K's fragments
     uint32_t q[NT][C::K16][2];
@@ -888,9 +933,6 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
       }
-      __syncwarp();
-      fetch();  // into K's place
-
       const int key0 = step * C::KEYS;
       const bool masked = key0 + C::KEYS - 1 > first_limit;
       float mx[NT][2];
@@ -919,7 +961,9 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       bool move = false;
 #pragma unroll
       for (int i = 0; i < NT; ++i) move |= mx[i][0] > m[i][0] + 1.f || mx[i][1] > m[i][1] + 1.f;
-      if (__any_sync(0xffffffffu, move)) {
+      move = __any_sync(0xffffffffu, move);
+      fetch(0);  // into K's place: by now every lane has its scores, so all of K has been read
+      if (move) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           float f[2];
@@ -992,8 +1036,9 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
       }
-      __syncwarp();
-      fetch();  // into V's place
+      // Into V's place, which every lane has read once it has a sum that its last fragment went into.  The vote waits for
+      // that; which lane then issues the load is all the same.
+      fetch(__any_sync(0xffffffffu, o[NT - 1][C::K16 - 1][0] == -1.23456789e-30f) ? 1 : 0);
     }
 
     // ---- this warp's part: O / l and the log-sum-exp
@@ -1080,7 +1125,7 @@ attn_prefix_combine_kernel(const __grid_constant__ PrefixParams p) {
 // How a call is divided.
 struct Sizes {
   int rows_own, blocks_p, units_p, tiles_p, cluster, splits;
-  int by_rows, blocks_own, own_slot, units_own, pieces;
+  int by_rows, blocks_own, own_slot, units_own, pieces, least;
   int64_t own_parts, row_slots, cum_bytes, bytes;
 };
 
@@ -1116,15 +1161,17 @@ bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Size
   const int64_t units = S ? static_cast<int64_t>(B) * Hkv * z.blocks_own : 0, steps = units * ((S + 15ll) / 16 + Y_START);
   if (steps > INT32_MAX / 16 || static_cast<int64_t>(z.units_p) * z.cluster * z.splits > INT32_MAX / 2) return false;
   z.units_own = static_cast<int>(units);
-  // every warp of two CTAs per SM has a piece, but a unit no more than 32: whoever adds them goes through all of them
-  z.pieces = 0;
+  // every warp of two CTAs per SM has a piece, but the longest unit no more parts than those that add them have room for:
+  // one for each piece that it fills, and two that it fills in part
+  z.pieces = 0, z.least = 1;
   if (z.by_rows && S) {
-    const int64_t warps = 2ll * sms * Y_WARPS, most = steps < 32 * units ? steps : 32 * units;
-    z.pieces = static_cast<int>(most < warps ? most : warps);
+    const int64_t warps = 2ll * sms * Y_WARPS;
+    z.pieces = static_cast<int>(steps < warps ? steps : warps);
+    z.least = static_cast<int>(((S + 15ll) / 16 + Y_START + OWN_PARTS - 2) / (OWN_PARTS - 1));
   }
   z.own_parts = z.splits > 1 ? static_cast<int64_t>(z.units_p) * z.splits * X_ROWS : 0;
   z.row_slots = z.own_parts + (units + z.pieces) * z.own_slot;
-  z.cum_bytes = (static_cast<int64_t>(B) * 4 + 4 + 15) / 16 * 16;
+  z.cum_bytes = (static_cast<int64_t>(B) * 8 + 4 + 15) / 16 * 16;
   z.bytes = z.cum_bytes + z.row_slots * (d + 1) * 4;
   return true;
 }
@@ -1138,7 +1185,8 @@ int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p,
     const void* fn = z.own_slot <= 8 ? reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 1>)
                                      : reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 2>);
     constexpr int ring = Y_WARPS * Own::SLOTS * Own::SLOT_BYTES + 1024;
-    if (allow_smem(fn, ring)) return WK_E_CUDA;
+    // all of the SM's shared memory, so that a CTA of the prefix kernel fits beside
+    if (allow_smem(fn, ring) || prefer_smem(fn)) return WK_E_CUDA;
     if (int bad = launch_pdl(fn, dim3((z.pieces + Y_WARPS - 1) / Y_WARPS), 32 * Y_WARPS, ring, stream, 1,
                              {const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]), &p}))
       return bad;
@@ -1151,7 +1199,7 @@ int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p,
   }
   if (z.units_p) {
     const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH, false>);
-    if (allow_smem(fn, C::SMEM) || allow_large_clusters(fn)) return WK_E_CUDA;
+    if (allow_smem(fn, C::SMEM) || allow_large_clusters(fn) || prefer_smem(fn)) return WK_E_CUDA;
     if (int bad = launch_pdl(fn, dim3(z.units_p * z.splits * z.cluster), X_THREADS, C::SMEM, stream, z.cluster,
                              {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]), &p}))
       return bad;
@@ -1231,10 +1279,10 @@ extern "C" int wk_attn_fwd_shared_prefix(const wk_attn_prefix_args* a, void* str
   p.B = a->B, p.Hq = a->Hq, p.Hkv = a->Hkv, p.group = a->Hq / a->Hkv, p.Nq = a->Nq, p.P = a->P, p.S = a->S;
   p.rows_own = z.rows_own, p.rows_all = z.rows_own * a->B;
   p.blocks_p = z.blocks_p, p.tiles_p = z.tiles_p, p.cluster = z.cluster, p.splits = z.splits;
-  p.by_rows = z.by_rows, p.blocks_own = z.blocks_own, p.own_slot = z.own_slot, p.pieces = z.pieces, p.own_parts = z.own_parts;
+  p.by_rows = z.by_rows, p.blocks_own = z.blocks_own, p.own_slot = z.own_slot, p.pieces = z.pieces, p.least = z.least, p.own_parts = z.own_parts;
   p.causal = a->causal, p.lse_natural = a->lse_natural;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  p.cum = static_cast<int*>(a->workspace);
+  p.cum = static_cast<int*>(a->workspace), p.lengths = p.cum + a->B + 1;
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + z.cum_bytes);
   p.part_lse = p.part + z.row_slots * a->d;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

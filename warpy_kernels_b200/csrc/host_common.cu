@@ -146,6 +146,10 @@ int allow_smem(const void* func, int bytes) {
   return set_once(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+int prefer_smem(const void* func) {
+  return set_once(func, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 int allow_large_clusters(const void* func) { return set_once(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); }
 
 int clusters_at_once(const void* func, int size, int threads, int smem) {

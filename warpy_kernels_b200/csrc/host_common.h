@@ -33,6 +33,10 @@ int sm_count();
 // Raises the dynamic shared memory limit of `func` once per device.
 int allow_smem(const void* func, int bytes);
 
+// Has an SM that runs `func` divide its memory for as much shared memory as there is, once per device: what is divided for
+// a first kernel's needs alone cannot take in another kernel's CTAs while the first one runs.
+int prefer_smem(const void* func);
+
 // Lets `func` be launched in clusters of up to 16 CTAs, once per device.
 int allow_large_clusters(const void* func);
 
