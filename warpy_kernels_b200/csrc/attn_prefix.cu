@@ -184,8 +184,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// Four e4m3 codes -> two words of bf16 pairs, exact.  The code's exponent and mantissa moved to where bf16 has them are
-// the value times 2^-120, subnormals included; one product puts that right.  The NaN codes would come out as 480.
+// Four e4m3 codes -> two words of bf16 pairs, exact but for the NaN codes, which come out as 480.  The code's exponent and
+// mantissa moved to where bf16 has them are the value times 2^-120, subnormals included; one product puts that right.
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   uint32_t x[2] = {__byte_perm(w, 0, 0x1404), __byte_perm(w, 0, 0x3424)};  // codes in the high bytes of the halves
 #pragma unroll
@@ -193,12 +193,15 @@ __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_
     x[i] = (x[i] & 0x80008000u) | ((x[i] >> 4) & 0x07f007f0u);
     x[i] = mul_bf16x2(x[i], 0x7b807b80u);  // 2^120
   }
-  if ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (((w >> (8 * i)) & 0x7f) == 0x7f) x[i / 2] |= 0x7fffu << (16 * (i & 1));
-  }
   lo = x[0], hi = x[1];
+}
+// Not zero if one of four codes is NaN (0x7f or 0xff).
+__device__ __forceinline__ uint32_t e4m3x4_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Puts NaN where the codes have it.
+__device__ __forceinline__ void restore_nan(uint32_t w, uint32_t& lo, uint32_t& hi) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (((w >> (8 * i)) & 0x7f) == 0x7f) (i < 2 ? lo : hi) |= 0x7fffu << (16 * (i & 1));
 }
 
 // OWN: the rows of one sequence over its own keys, one CTA for 128 rows, which leaves a part.  Else: stacked rows over the
@@ -455,7 +458,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           const int row = r >> 1;
           const uint32_t src = smem + C::V_AT + st * C::K_BYTES + row * 128;
           const uint32_t dst = smem + C::V16_AT + grp * C::V16_BYTES + row * 128;
-          const bool there = key0 + row < keys;
+          const bool behind = key0 + row >= keys;
 #pragma unroll
           for (int c = 0; c < HALF; ++c) {
             const int piece = (r & 1) * HALF + c;
@@ -463,8 +466,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                          : "r"(src + ((piece ^ (row & 7)) << 4)));
+            if (behind) w[0] = w[1] = w[2] = w[3] = 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) e4m3x4_to_bf16(there ? w[x] : 0u, o[2 * x], o[2 * x + 1]);
+            for (int x = 0; x < 4; ++x) e4m3x4_to_bf16(w[x], o[2 * x], o[2 * x + 1]);
+            if (e4m3x4_nan(w[0]) | e4m3x4_nan(w[1]) | e4m3x4_nan(w[2]) | e4m3x4_nan(w[3])) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) restore_nan(w[x], o[2 * x], o[2 * x + 1]);
+            }
             const uint32_t to = dst + (piece >> 2) * C::KV_SPAN;
             const int at = (2 * piece) & 7;
             sts128(to + ((at ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
@@ -658,7 +666,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // Keys play the 16-row side of the MMAs and the rows the 8-column side, once or twice:
 //   S^T[16 keys, 8 rows] = K.Q^T     O^T[d, 8 rows] += V^T.P^T
 // so that a sequence's few rows leave little of an MMA empty and the accumulators take half the registers.  Tiles of K and V
-// come in turn by TMA into a ring of the warp's own (three times 4 KiB) and go to the MMAs by ldmatrix; P changes lanes with
+// come in turn by TMA into a ring of the warp's own (three or six times 4 KiB) and go to the MMAs by ldmatrix; P changes lanes with
 // movmatrix.  FP8: ldmatrix moves pairs of codes; which index of the head dimension a pair stands for is the same for K and
 // Q, and only moves O's rows for V.
 //
@@ -696,14 +704,16 @@ __device__ __forceinline__ void sum_weights(const PrefixParams& p, int* cum, int
   __syncthreads();
 }
 
-template <bool FP8, int DH>
+template <bool FP8, int DH, int NT>
 struct OwnCfg {
   static constexpr int SIZE = FP8 ? 1 : 2;
   static constexpr int SPANS = DH * SIZE > 128 ? 2 : 1;  // 128-byte spans of a row (FP8, 64: the upper half is zeros)
   static constexpr int KEYS = 32 / SPANS;                // of a step
   static constexpr int SPAN_BYTES = KEYS * 128;
   static constexpr int SLOT_BYTES = SPANS * SPAN_BYTES;  // 4 KiB
-  static constexpr int SLOTS = 3;
+  // Of the ring.  Units of 8 rows run in two CTAs per SM beside one of the prefix kernel, and their rings fill the shared
+  // memory that it leaves; units of 16 rows in one.
+  static constexpr int SLOTS = NT == 1 ? 3 : 6;
   static constexpr int K16 = DH / 16;                    // MMAs over the head dimension
   static constexpr float P_SHIFT = FP8 ? 14.f : 0.f;     // P is stored times 2^14
 };
@@ -804,7 +814,7 @@ template <bool FP8, int DH, int NT>
 __global__ void __launch_bounds__(32 * Y_WARPS) __maxnreg__(NT == 1 ? 112 : 168)
 attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ PrefixParams p) {
-  using C = OwnCfg<FP8, DH>;
+  using C = OwnCfg<FP8, DH, NT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int cum_mem[Y_CUM + 1], length_mem[Y_CUM], warp_sums[Y_WARPS];
   __shared__ __align__(8) uint64_t bar_mem[Y_WARPS][C::SLOTS];
@@ -1130,16 +1140,20 @@ struct Sizes {
 };
 
 // CTAs of a cluster and clusters of a unit.  A CTA is taken to cost a start and end (more in a larger cluster), and its
-// tiles, which go faster where it has an SM to itself; clusters of a unit beyond one cost the kernel that adds them up.
+// tiles, which go faster where it has an SM to itself; clusters of a unit beyond one cost the kernel that adds them up.  A
+// cluster lies within a group of SMs, of which larger ones leave some idle: with one CTA per SM 74 clusters of 2, 33 of 4, 15
+// of 8 and 7 of 16 run at once.
 void divide_prefix(int sms, Sizes& z) {
   double best = 0;
   for (int cluster = 1; cluster <= X_CLUSTER; cluster *= 2)
     for (int splits = 1; splits <= 16; splits *= 2) {
       const int64_t shares = static_cast<int64_t>(cluster) * splits;
       if (shares > 1 && (shares > z.tiles_p || (splits > 1 && cluster < 8))) continue;
-      const int64_t ctas = z.units_p * shares, waves = (ctas + 2 * sms - 1) / (2 * sms);
+      const int64_t ctas = z.units_p * shares;
+      const int64_t at_once = sms * (cluster <= 2 ? 148 : cluster == 4 ? 132 : cluster == 8 ? 120 : 112) / 148;
+      const int64_t waves = (ctas + 2 * at_once - 1) / (2 * at_once);
       const double tiles = static_cast<double>((z.tiles_p + shares - 1) / shares);
-      const double cost = waves * (4.0 + 0.15 * cluster + tiles * (ctas <= sms ? 0.65 : 1.1)) + (splits > 1 ? 4.0 : 0.0);
+      const double cost = waves * (4.0 + 0.15 * cluster + tiles * (ctas <= at_once ? 0.65 : 1.1)) + (splits > 1 ? 4.0 : 0.0);
       if (shares == 1 || cost < best) best = cost, z.cluster = cluster, z.splits = splits;
     }
 }
@@ -1161,11 +1175,12 @@ bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Size
   const int64_t units = S ? static_cast<int64_t>(B) * Hkv * z.blocks_own : 0, steps = units * ((S + 15ll) / 16 + Y_START);
   if (steps > INT32_MAX / 16 || static_cast<int64_t>(z.units_p) * z.cluster * z.splits > INT32_MAX / 2) return false;
   z.units_own = static_cast<int>(units);
-  // every warp of two CTAs per SM has a piece, but the longest unit no more parts than those that add them have room for:
+  // every warp that runs at once has a piece, but the longest unit no more parts than those that add them have room for:
   // one for each piece that it fills, and two that it fills in part
   z.pieces = 0, z.least = 1;
   if (z.by_rows && S) {
-    const int64_t warps = 2ll * sms * Y_WARPS;
+    // of two CTAs per SM; of one where units of 16 rows leave room for no more beside a CTA of the prefix kernel
+    const int64_t warps = (z.own_slot > 8 && z.units_p ? 1ll : 2ll) * sms * Y_WARPS;
     z.pieces = static_cast<int>(steps < warps ? steps : warps);
     z.least = static_cast<int>(((S + 15ll) / 16 + Y_START + OWN_PARTS - 2) / (OWN_PARTS - 1));
   }
@@ -1181,10 +1196,12 @@ int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p,
   using C = PrefixCfg<FP8, DH>;
   static_assert(2 * (C::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
   if (z.units_own && z.by_rows) {
-    using Own = OwnCfg<FP8, DH>;
-    const void* fn = z.own_slot <= 8 ? reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 1>)
-                                     : reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 2>);
-    constexpr int ring = Y_WARPS * Own::SLOTS * Own::SLOT_BYTES + 1024;
+    const bool narrow = z.own_slot <= 8;
+    const void* fn = narrow ? reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 1>)
+                            : reinterpret_cast<const void*>(attn_prefix_own_kernel<FP8, DH, 2>);
+    using N1 = OwnCfg<FP8, DH, 1>;
+    using N2 = OwnCfg<FP8, DH, 2>;
+    const int ring = Y_WARPS * (narrow ? N1::SLOTS * N1::SLOT_BYTES : N2::SLOTS * N2::SLOT_BYTES) + 1024;
     // all of the SM's shared memory, so that a CTA of the prefix kernel fits beside
     if (allow_smem(fn, ring) || prefer_smem(fn)) return WK_E_CUDA;
     if (int bad = launch_pdl(fn, dim3((z.pieces + Y_WARPS - 1) / Y_WARPS), 32 * Y_WARPS, ring, stream, 1,
