@@ -811,7 +811,7 @@ __device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) {
 
 // NT: groups of eight rows, 1 or 2.
 template <bool FP8, int DH, int NT>
-__global__ void __launch_bounds__(32 * Y_WARPS) __maxnreg__(NT == 1 ? 112 : 168)
+__global__ void __maxnreg__(NT == 1 ? 112 : 168)
 attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ PrefixParams p) {
   using C = OwnCfg<FP8, DH, NT>;
