@@ -12,7 +12,7 @@
 // few, where heads are fewer than the rows it holds; a part of the heads, where tokens are few), so that an angle is made
 // once for the heads of its token and its products with the weights stay in registers.  A warp goes on to the next tokens by
 // itself; every lane fetches its own pieces a few rows ahead, across tokens, with cp.async into a ring of its own, so that
-// loads are under way while angles are made; a warp does its share of the queries, then of the keys.
+// loads are under way while angles are made.
 //
 // Angles: position times inv_freq in turns, reduced to half a turn in fp64 (positions beyond 2^20 leave nothing of an fp32
 // product's fraction), then sine and cosine in fp32.
@@ -82,12 +82,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 template <typename T>
 constexpr int kRowBytes = 512 * sizeof(T);
 template <typename T>
-__device__ __forceinline__ void fetch_raw(uint32_t dst, const T* p, int at_a, int at_b) {
-  cp_async16(dst, p + at_a);
-  cp_async16(dst + 512, p + at_b);
+__device__ __forceinline__ void fetch_raw(uint32_t dst, const T* p, int between) {
+  cp_async16(dst, p);
+  cp_async16(dst + 512, p + between);
   if (sizeof(T) == 4) {
-    cp_async16(dst + 1024, p + at_a + 4);
-    cp_async16(dst + 1536, p + at_b + 4);
+    cp_async16(dst + 1024, p + 4);
+    cp_async16(dst + 1536, p + between + 4);
   }
 }
 template <typename T>
@@ -340,27 +340,21 @@ __device__ __forceinline__ float dot(const uint64_t (&a)[8], const uint64_t (&b)
   return sum_of(add_f32x2(x, y));
 }
 
-// The groups of tokens that a warp works through, first for the queries, then for the keys; it takes one of the `hs` shares
-// of their heads.  hs divides the number of warps, so that neither the share nor the distance to the next group changes, and
-// the keys' groups go round from where the queries' ended.
+// The groups of tokens that a warp works through; it takes one of the `hs` shares of their heads.  hs divides the number of
+// warps, so that neither the share nor the distance to the next group changes.
 template <int LPR>
 struct Walk {
-  int side, group, groups, group_step;
+  int group, groups, group_step;
   int token, b, n, token_step, b_step, n_step;  // of this lane
   __device__ __forceinline__ Walk(const RopeParams& p, const Place<LPR>& at) {
     group_step = gridDim.x * (kThreads / 32) / p.hs;
     groups = (p.tokens + p.tb - 1) / p.tb;
     token_step = group_step * p.tb;
     b_step = token_step / p.N, n_step = token_step - b_step * p.N;
-    begin(p, at, 0);
+    begin(p, at);
   }
-  __device__ __forceinline__ void begin(const RopeParams& p, const Place<LPR>& at, int which) {
-    side = which;
+  __device__ __forceinline__ void begin(const RopeParams& p, const Place<LPR>& at) {
     group = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) / p.hs;
-    if (side) {
-      const int behind = groups % group_step;
-      group += group < behind ? group_step - behind : -behind;
-    }
     token = group * p.tb + at.tslot;
     b = token / p.N, n = token - b * p.N;
   }
@@ -372,55 +366,64 @@ struct Walk {
 };
 
 // The rows that a lane fetches ahead into its ring: two heads at a step, `hb` apart, of IN tensors (backward: also the
-// gradients).
+// gradients).  Forward: the queries and then the keys of a group of tokens.  Backward: the queries of all groups, then the
+// keys, so that one weight's gradient is summed at a time.
 template <typename T, int LPR, bool BWD>
 struct Fetcher {
   static constexpr int IN = BWD ? 2 : 1, STAGES = kStages<T, BWD>, BYTES = 2 * IN * kRowBytes<T>;
   Walk<LPR> walk;
   uint32_t ring;
-  int h, first, every, heads;
+  int side, h, first, every, heads, between;
+  bool live, more;  // the lane's token exists; something is left to fetch
   const T* from[IN];
-  int64_t apart[IN];  // of the two heads
+  int64_t apart[IN], next[IN];  // of the two heads, of the steps
   __device__ __forceinline__ Fetcher(const RopeParams& p, const Place<LPR>& at, uint32_t ring, int first)
-      : walk(p, at), ring(ring), first(first), every(2 * p.hs * p.hb) {
-    side(p);
-    if (!walk.here()) go_on(p, at);
+      : walk(p, at), ring(ring), side(0), first(first), every(2 * p.hs * p.hb), between(at.at_b - at.at_a), more(true) {
+    start(p, at);
   }
-  __device__ __forceinline__ void side(const RopeParams& p) {
-    heads = p.heads[walk.side];
-    apart[0] = p.hb * p.xs[walk.side][1];
-    if (BWD) apart[IN - 1] = p.hb * p.dys[walk.side][1];
-    start(p);
+  // The first step of the side, or of the next one that has any for this warp.
+  __device__ __forceinline__ void start(const RopeParams& p, const Place<LPR>& at) {
+    while (!walk.here() || first - at.hslot >= p.heads[side])
+      if (!advance(p, at)) return;
+    h = first, heads = p.heads[side];
+    live = at.active && walk.token < p.tokens;
+#pragma unroll
+    for (int i = 0; i < IN; ++i) {
+      const int64_t(&st)[3] = i ? p.dys[side] : p.xs[side];
+      from[i] = static_cast<const T*>(i ? p.dy[side] : p.x[side]) + walk.b * st[0] + walk.n * st[2] + first * st[1] + at.at_a;
+      apart[i] = p.hb * st[1], next[i] = 2 * p.hs * apart[i];
+    }
   }
-  __device__ __forceinline__ void start(const RopeParams& p) {
-    const int w = walk.side;
-    h = first;
-    from[0] = static_cast<const T*>(p.x[w]) + walk.b * p.xs[w][0] + walk.n * p.xs[w][2] + first * p.xs[w][1];
-    if (BWD)
-      from[IN - 1] = static_cast<const T*>(p.dy[w]) + walk.b * p.dys[w][0] + walk.n * p.dys[w][2] + first * p.dys[w][1];
-  }
-  // To the keys, once the queries are through.
-  __device__ __forceinline__ void go_on(const RopeParams& p, const Place<LPR>& at) {
-    if (walk.side || !p.heads[1]) return;
-    walk.begin(p, at, 1);
-    side(p);
+  __device__ __forceinline__ bool advance(const RopeParams& p, const Place<LPR>& at) {
+    if (BWD) {
+      if (walk.here()) walk.next(p);
+      if (walk.here()) return true;
+      if (side || !p.heads[1]) return more = false;
+      side = 1;
+      walk.begin(p, at);
+      return true;
+    }
+    if (!walk.here()) return more = false;
+    if (!side && p.heads[1]) {
+      side = 1;
+    } else {
+      side = 0;
+      walk.next(p);
+    }
+    return true;
   }
   __device__ __forceinline__ void operator()(const RopeParams& p, const Place<LPR>& at, int stage) {
-    if (walk.here()) {
-      const int there = at.active && walk.token < p.tokens ? heads - h : 0;
+    if (more) {
+      const int there = live ? heads - h : 0;
 #pragma unroll
       for (int i = 0; i < IN; ++i) {
         const uint32_t dst = ring + stage * BYTES + 2 * i * kRowBytes<T>;
-        if (there > 0) fetch_raw(dst, from[i], at.at_a, at.at_b);
-        if (there > p.hb) fetch_raw(dst + kRowBytes<T>, from[i] + apart[i], at.at_a, at.at_b);
-        from[i] += 2 * p.hs * apart[i];
+        if (there > 0) fetch_raw(dst, from[i], between);
+        if (there > p.hb) fetch_raw(dst + kRowBytes<T>, from[i] + apart[i], between);
+        from[i] += next[i];
       }
       h += every;
-      if (h - at.hslot >= heads) {  // the same for the whole warp
-        walk.next(p);
-        if (walk.here()) start(p);
-        else go_on(p, at);
-      }
+      if (h - at.hslot >= heads && advance(p, at)) start(p, at);  // the same for the whole warp
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
@@ -434,39 +437,52 @@ rope_kernel(const __grid_constant__ RopeParams p) {
   constexpr int WARPS = kThreads / 32;
   extern __shared__ __align__(16) uint8_t ring_mem[];
   __shared__ __align__(16) float tables[WARPS][kTable];
+  __shared__ __align__(16) float weights[NORM ? 2 * kMaxD : 4];
   const int warp = threadIdx.x / 32;
   const uint32_t ring = smem_u32(ring_mem) + warp * Fetch::STAGES * Fetch::BYTES + (threadIdx.x % 32) * 16;
   const Place<LPR> at(p);
   const float inv_d = 1.f / static_cast<float>(p.d);
   const int first = (blockIdx.x * WARPS + warp) % p.hs * 2 * p.hb + at.hslot, every = 2 * p.hs * p.hb;
+  const int sides = p.heads[1] ? 2 : 1;
   pdl_launch_dependents();
   pdl_wait();
 
   Fetch fetch(p, at, ring, first);
   for (int i = 0; i < Fetch::STAGES; ++i) fetch(p, at, i);
+  if (NORM) {
+    for (int i = threadIdx.x * 8; i < sides * p.d; i += kThreads * 8) weight8(p.w[i >= p.d], p.w_dtype, i >= p.d ? i - p.d : i, weights + i);
+    __syncthreads();
+  }
   int stage = 0;
   Walk<LPR> now(p, at);
-  for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
-    if (side) now.begin(p, at, 1);
-    const int heads = p.heads[side];
-    float w[16];
+  for (; now.here(); now.next(p)) {
+    const bool live = at.active && now.token < p.tokens;
+    float c[8], s[8];
+    angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
+    uint64_t own[8], other[8];
+    if (!NORM) {
+      float w[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = 1.f;
-    if (NORM && at.active && now.here()) {
-      weight8(p.w[side], p.w_dtype, at.at_a, w);
-      weight8(p.w[side], p.w_dtype, at.at_b, w + 8);
+      for (int i = 0; i < 16; ++i) w[i] = 1.f;
+      factors(c, s, w, at.turned, p.interleaved, own, other);
     }
-    const int64_t apart = p.hb * p.ys[side][1];
-    for (; now.here(); now.next(p)) {
-      uint64_t own[8], other[8];
-      const bool live = at.active && now.token < p.tokens;
-      {
-        float c[8], s[8];
-        angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
+    for (int side = 0; side < sides; ++side) {
+      const int heads = p.heads[side];
+      if (NORM && at.active) {
+        float w[16];
+        const float* from = weights + side * p.d;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 x = reinterpret_cast<const float4*>(from + at.at_a)[i], y = reinterpret_cast<const float4*>(from + at.at_b)[i];
+          w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+          w[8 + 4 * i] = y.x, w[9 + 4 * i] = y.y, w[10 + 4 * i] = y.z, w[11 + 4 * i] = y.w;
+        }
         factors(c, s, w, at.turned, p.interleaved, own, other);
       }
-      Out* to = static_cast<Out*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
-      for (int h = first; h - at.hslot < heads; h += every, to += 2 * p.hs * apart) {
+      const int64_t apart = p.hb * p.ys[side][1], next = 2 * p.hs * apart;
+      const int between = at.at_b - at.at_a;
+      Out* to = static_cast<Out*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1] + at.at_a;
+      for (int h = first; h - at.hslot < heads; h += every, to += next) {
         const int there = live ? heads - h : 0;
         float scale[2] = {1.f, 1.f};
         if (FP8) {
@@ -501,8 +517,9 @@ rope_kernel(const __grid_constant__ RopeParams p) {
             for (int j = 0; j < 8; ++j) y[j] = mul_f32x2(y[j], f2);
           }
           if (there > i * p.hb) {
-            store8(to + i * apart + at.at_a, y);
-            store8(to + i * apart + at.at_b, y + 4);
+            Out* dst = i ? to + apart : to;
+            store8(dst, y);
+            store8(dst + between, y + 4);
           }
         }
         fetch(p, at, stage);  // into the place that has just been read
@@ -533,7 +550,7 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
   int stage = 0;
   Walk<LPR> now(p, at);
   for (int side = 0; side < (p.heads[1] ? 2 : 1); ++side) {
-    if (side) now.begin(p, at, 1);
+    if (side) now.begin(p, at);
     const int heads = p.heads[side];
     uint64_t w[8], dw[8];
     {
@@ -545,13 +562,14 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = pack_f32x2(v[2 * i], v[2 * i + 1]), dw[i] = 0;
     }
-    const int64_t apart = p.hb * p.ys[side][1];
-    for (; now.here(); now.next(p)) {
+    const int64_t apart = p.hb * p.ys[side][1], next = 2 * p.hs * apart;
+    const int between = at.at_b - at.at_a;
+    for (; now.here() && first - at.hslot < heads; now.next(p)) {
       const bool live = at.active && now.token < p.tokens;
       float c[8], s[8];
       angles<T, LPR>(p, at, live, now.b, now.n, tables[warp], c, s);
-      T* to = static_cast<T*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1];
-      for (int head = first; head - at.hslot < heads; head += every, to += 2 * p.hs * apart) {
+      T* to = static_cast<T*>(p.y[side]) + now.b * p.ys[side][0] + now.n * p.ys[side][2] + first * p.ys[side][1] + at.at_a;
+      for (int head = first; head - at.hslot < heads; head += every, to += next) {
         const int there = live ? heads - head : 0;
         asm volatile("cp.async.wait_group %0;" ::"n"(Fetch::STAGES - 1) : "memory");
 #pragma unroll
@@ -578,8 +596,9 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
               dw[j] = fma_f32x2(mul_f32x2(g[j], x[j]), f2, dw[j]);
               h[j] = fma_f32x2(x[j], m2, mul_f32x2(h[j], f2));
             }
-            store8(to + i * apart + at.at_a, h);
-            store8(to + i * apart + at.at_b, h + 4);
+            T* dst = i ? to + apart : to;
+            store8(dst, h);
+            store8(dst + between, h + 4);
           }
         }
         fetch(p, at, stage);
@@ -644,28 +663,32 @@ dweight_kernel(const float* __restrict__ partial, int parts, int d, void* dw_q, 
     static_cast<__half*>(out)[col] = __float2half_rn(s);
 }
 
-// How a warp's rows are divided into heads and tokens: the division that takes the fewest instructions per token (150 for a
-// step over two rows per lane, 40 for an angle, 60 for a group of tokens), and over how many warps the heads of a token are
-// spread: so many (of those that divide the warps of a CTA) that the last round of the groups over the warps costs least.
-void divide(RopeParams& p, int ctas_at_once, int& ctas) {
-  const int lpr = p.d / 16, rows = 32 / lpr, pairs = p.rot / 2, warps = kThreads / 32, sides = p.heads[1] ? 2 : 1;
+// How a warp's rows are divided into heads and tokens: the division that takes the fewest instructions per token (300 for a
+// step over two rows per lane, 40 for an angle, 150 for a group of tokens), weighed with how short the pieces of memory are
+// that it reads at a time: neighbouring heads of a token, or neighbouring tokens of a head, whichever lie side by side.
+// (4 x 4096 tokens, 32 / 8 heads, d 128, heads side by side, bf16: 4 heads and one token at a time 60.4 us, 2 and 2 65.4,
+// 1 and 4 66.2; 16385 tokens, 16 / 16 heads, d 80, fp16: 3 and 2 38.2 us, 2 and 3 41.6, 1 and 6 44.9.)
+// And over how many warps the heads of a token are spread: so many (of those that divide the warps of a CTA) that the last
+// round of the groups over the warps costs least.
+void divide(RopeParams& p, int ctas_at_once, int size, int& ctas) {
+  const int lpr = p.d / 16, rows = 32 / lpr, pairs = p.rot / 2, warps = kThreads / 32;
   auto steps = [&](int side, int hb) { return (p.heads[side] + 2 * hb - 1) / (2 * hb); };
   double best = 0, fixed = 0;
   for (int hb = 1; hb <= rows; ++hb) {
-    const double f = 60.0 + 40.0 * ((pairs + hb * lpr - 1) / (hb * lpr));
-    const double cost = (150.0 * (steps(0, hb) + steps(1, hb)) + sides * f) / (rows / hb);
-    if (hb == 1 || cost < best) best = cost, fixed = f, p.hb = hb, p.tb = rows / hb;
+    const int tb = rows / hb;
+    const double f = 150.0 + 40.0 * ((pairs + hb * lpr - 1) / (hb * lpr));
+    const int side_by_side = p.xs[0][1] == p.d ? 2 * hb : p.xs[0][2] == p.d ? tb : 1;
+    const double cost = (300.0 * (steps(0, hb) + steps(1, hb)) + f) / tb * (1.0 + 420.0 / (side_by_side * p.d * size));
+    if (hb == 1 || cost < best) best = cost, fixed = f, p.hb = hb, p.tb = tb;
   }
   const int64_t groups = (p.tokens + p.tb - 1) / p.tb;
   for (int hs = 1; hs <= warps && hs < 2 * steps(0, p.hb); hs *= 2) {
-    double cost = 0;
-    for (int side = 0; side < sides; ++side) {
-      const double rounds = static_cast<double>(groups * hs) / (static_cast<double>(ctas_at_once) * warps);
-      cost += (rounds < 1 ? 1 : rounds > 4 ? rounds : ceil(rounds)) * (fixed + 150.0 * ((steps(side, p.hb) + hs - 1) / hs));
-    }
+    const double rounds = static_cast<double>(groups * hs) / (static_cast<double>(ctas_at_once) * warps);
+    const double work = fixed + 300.0 * ((steps(0, p.hb) + hs - 1) / hs + (steps(1, p.hb) + hs - 1) / hs);
+    const double cost = (rounds < 1 ? 1 : rounds > 4 ? rounds : ceil(rounds)) * work;
     if (hs == 1 || cost < best) best = cost, p.hs = hs;
   }
-  const int64_t want = (groups * p.hs * sides + warps - 1) / warps;
+  const int64_t want = (groups * p.hs + warps - 1) / warps;
   ctas = static_cast<int>(want < ctas_at_once ? want : ctas_at_once);
 }
 
@@ -770,7 +793,7 @@ extern "C" int wk_rope(const wk_rope_args* a, void* stream) {
                                             : forward_kernel<float>(p.d, fp8, norm);
   const int smem = a->dtype == WK_F32 ? kRingBytes<float, false> : kRingBytes<__half, false>;
   int ctas;
-  divide(p, ctas_at_once(sms, smem, kTableBytes), ctas);
+  divide(p, ctas_at_once(sms, smem, kTableBytes + 2 * kMaxD * 4), elem_size(a->dtype), ctas);
   if (allow_smem(kernel, smem)) return WK_E_CUDA;
   return launch_pdl(kernel, dim3(ctas), kThreads, smem, static_cast<cudaStream_t>(stream), 1, {&p});
 }
@@ -795,7 +818,7 @@ extern "C" int wk_qk_norm_rope_bwd(const wk_rope_args* a, void* stream) {
                                             : backward_kernel<float>(p.d);
   const int smem = a->dtype == WK_F32 ? kRingBytes<float, true> : kRingBytes<__half, true>;
   int ctas;
-  divide(p, ctas_at_once(sms, smem, kTableBytes + kSumBytes), ctas);
+  divide(p, ctas_at_once(sms, smem, kTableBytes + kSumBytes), elem_size(a->dtype), ctas);
   if (allow_smem(kernel, smem)) return WK_E_CUDA;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int bad = launch_pdl(kernel, dim3(ctas), kThreads, smem, st, 1, {&p})) return bad;
