@@ -161,6 +161,35 @@ def test_nan_where_it_is_seen(cuda, fp8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("S", [0, 200])
+@pytest.mark.parametrize("Nq", [1, 9, 40])  # own keys by 8 and 16 rows at a time, and by tiles
+def test_keys_whose_scores_are_minus_infinity(cuda, Nq, S):
+    """They count nothing, also where a segment starts with them; a row that sees nothing else gets 0 and +inf."""
+    B, Hq, Hkv, P, d = 3, 4, 2, 300, 128
+    t = make(B, Hq, Hkv, Nq, P, S, d, False)
+    t["q"].abs_()
+    for n, count in (("k_prefix", 170), ("k", 70)):
+        t[n][:, :, :count] = float("-inf")
+    got = wk.attn_fwd_shared_prefix(**t)
+    less = dict(t) | {n: t[n][:, :, 170:] for n in ("k_prefix", "v_prefix")} | {n: t[n][:, :, 70:] for n in "kv"}
+    check(less, got)
+    t["k_prefix"][:], t["k"][1] = float("-inf"), float("-inf")
+    out, lse = wk.attn_fwd_shared_prefix(**t)
+    empty = [1] if S else [0, 1, 2]
+    assert not out[empty].any() and torch.isposinf(lse[empty]).all()
+    assert S == 0 or bool(lse[[0, 2]].isfinite().all())
+
+
+@pytest.mark.gpu
+def test_more_keys_than_are_counted(cuda):
+    """No workspace is large enough for them, and the call is refused."""
+    from warpy_kernels_b200 import _lib
+
+    size = _lib.lib().wk_attn_fwd_shared_prefix_workspace_bytes
+    assert size(1, 1, 1, 1, 1 << 29, 1 << 29, 64) == 0 and size(1, 1, 1, 1, 1 << 29, (1 << 29) - 1, 64) > 0
+
+
+@pytest.mark.gpu
 def test_codes_of_v(cuda):
     """Every e4m3 code of V through the conversion to bf16: one key has all the weight."""
     d = 128

@@ -144,7 +144,7 @@ def attn_fwd_shared_prefix(
     with torch.cuda.device(dev):
         args.workspace_bytes = lib.wk_attn_fwd_shared_prefix_workspace_bytes(B, Hq, Hkv, Nq, P, S, d)
     if args.workspace_bytes == 0:
-        raise ValueError("the problem has more than 2^30 query rows or 2^27 tiles of keys")
+        raise ValueError("the problem has more than 2^30 query rows, 2^30 keys of a sequence or 2^27 tiles of keys")
     workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=dev)
     args.workspace = workspace.data_ptr()
     entry = _lib.address(lib.wk_attn_fwd_shared_prefix)

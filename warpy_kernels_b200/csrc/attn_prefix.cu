@@ -1161,7 +1161,7 @@ void divide_prefix(int sms, Sizes& z) {
 // false if the problem is beyond the kernels' 32-bit counts.
 bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Sizes& z) {
   const int64_t rows_own = static_cast<int64_t>(Hq / Hkv) * Nq, rows_all = rows_own * B;
-  if (rows_all * Hkv > INT32_MAX / 2) return false;
+  if (rows_all * Hkv > INT32_MAX / 2 || static_cast<int64_t>(P) + S > INT32_MAX / 2) return false;
   z.rows_own = static_cast<int>(rows_own);
   z.blocks_p = static_cast<int>((rows_all + X_ROWS - 1) / X_ROWS);
   z.tiles_p = P / X_KEYS + (P % X_KEYS != 0);
