@@ -40,7 +40,9 @@ constexpr int X_SOFTMAX = 256;
 constexpr int X_TMEM_COLS = 256;
 constexpr int X_S_COLS = 64;  // buffer b at column 64 b; P over its first 32
 constexpr int X_O_COL = 128;
-constexpr float X_MAX_EXP = 60.f;
+// How far (as a power of two) a row may rise above its reference before the CTA goes through its keys again, and what P is
+// stored times: bf16 has the exponent range, f16 (FP8 inputs) needs a larger P for the small probabilities.
+constexpr float X_MAX_EXP = 60.f, X_MAX_EXP_F16 = 10.f, X_SHIFT_F16 = 5.f, X_SHIFT_AGAIN = 14.f;
 constexpr int X_CLUSTER = 16;  // largest cluster
 constexpr int X_PAD = 4;       // values between rows in the exchange: lanes with neighbouring rows write without conflicts
 
@@ -157,17 +159,18 @@ struct PrefixCfg {
   static constexpr int Q_BYTES = SPANS * Q_SPAN;
   static constexpr int K_BYTES = SPANS * KV_SPAN;      // of a stage; V as loaded likewise
   static constexpr int V16_BYTES = V_SPANS * KV_SPAN;
-  static constexpr int STAGES = FP8 ? 3 : DH == 64 ? 4 : 2;
+  static constexpr int STAGES = FP8 || DH == 128 ? 2 : 4;
+  static constexpr int V16S = 3;  // FP8: buffers of V in bf16
   static constexpr int Q_AT = 0;
   static constexpr int K_AT = Q_BYTES;
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
-  static constexpr int V16_AT = V_AT + STAGES * K_BYTES;  // FP8 only: two buffers
+  static constexpr int V16_AT = V_AT + STAGES * K_BYTES;  // FP8 only
   // row reference, then l and largest score of each group; at the end the log-sum-exp of each row
-  static constexpr int X_AT = V16_AT + (FP8 ? 2 * V16_BYTES : 0);
+  static constexpr int X_AT = V16_AT + (FP8 ? V16S * V16_BYTES : 0);
   static constexpr int ROW_AT = X_AT + 5 * X_ROWS * 4;  // where each row of Q is
   static constexpr int TARGET_AT = ROW_AT + X_ROWS * 8;
   static constexpr int BAR_AT = TARGET_AT + X_ROWS * static_cast<int>(sizeof(RowTarget));
-  static constexpr int SMEM = BAR_AT + 8 * (4 * STAGES + 8) + 16 + 1024;
+  static constexpr int SMEM = BAR_AT + 8 * (4 * STAGES + 7 + V16S) + 1024;
   // the exchange of a cluster takes the place of the tiles
   static constexpr int PART_BYTES = X_ROWS * (DH + X_PAD) * 4;
   static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowWeights)) <= X_AT, "");
@@ -179,31 +182,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// Four e4m3 codes -> two words of bf16 pairs, exact but for the NaN codes, which come out as 480.  The code's exponent and
-// mantissa moved to where bf16 has them are the value times 2^-120, subnormals included; one product puts that right.
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  uint32_t x[2] = {__byte_perm(w, 0, 0x1404), __byte_perm(w, 0, 0x3424)};  // codes in the high bytes of the halves
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    x[i] = (x[i] & 0x80008000u) | ((x[i] >> 4) & 0x07f007f0u);
-    x[i] = mul_bf16x2(x[i], 0x7b807b80u);  // 2^120
-  }
-  lo = x[0], hi = x[1];
-}
-// Not zero if one of four codes is NaN (0x7f or 0xff).
-__device__ __forceinline__ uint32_t e4m3x4_nan(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-// Puts NaN where the codes have it.
-__device__ __forceinline__ void restore_nan(uint32_t w, uint32_t& lo, uint32_t& hi) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (((w >> (8 * i)) & 0x7f) == 0x7f) (i < 2 ? lo : hi) |= 0x7fffu << (16 * (i & 1));
-}
-
 // OWN: the rows of one sequence over its own keys, one CTA for 128 rows, which leaves a part.  Else: stacked rows over the
 // prefix.
 template <bool FP8, int DH, bool OWN>
@@ -223,6 +201,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
   auto s_full = [&](int b) { return misc + 8u * b; };
   auto p_full = [&](int b) { return misc + 8u * (2 + b); };
   const uint32_t q_full = misc + 8u * 4, o_full = misc + 8u * 5, tmem_slot = misc + 8u * 6;
+  auto v16_empty = [&](int s) { return misc + 8u * (7 + s); };
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -238,6 +217,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     }
     mbar_init(q_full, X_SOFTMAX);
     mbar_init(o_full, 1);
+    for (int i = 0; i < C::V16S; ++i) mbar_init(v16_empty(i), 1);
     mbar_fence_init();
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
@@ -334,7 +314,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     } else if (warp == 1) {
       const bool mine = elect_one();
       constexpr uint32_t idesc_qk = FP8 ? make_idesc(0, 0, 0, 0, X_ROWS, X_KEYS) : make_idesc(1, 1, 0, 0, X_ROWS, X_KEYS);
-      constexpr uint32_t idesc_pv = make_idesc(1, 1, 0, 1, X_ROWS, DH);
+      constexpr uint32_t idesc_pv = make_idesc(!FP8, !FP8, 0, 1, X_ROWS, DH);
       const uint64_t q_desc = smem_desc_sw128(smem + C::Q_AT, 16, 1024);
       if (pass == 0) ok = mbar_wait_warp(q_full, 0, p.status, WK_ERR_TIMEOUT_LOAD);
       // the tensor pipe runs in issue order: the scores also wait for the product that last read their buffer
@@ -366,12 +346,12 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         if (!ok) break;
         tc_fence_after();
         const uint64_t v_desc = smem_desc_sw128(
-            FP8 ? smem + C::V16_AT + buf * C::V16_BYTES : smem + C::V_AT + st * C::K_BYTES, C::KV_SPAN, 1024);
+            FP8 ? smem + C::V16_AT + (J + j) % C::V16S * C::V16_BYTES : smem + C::V_AT + st * C::K_BYTES, C::KV_SPAN, 1024);
         if (mine) {
 #pragma unroll
           for (int k = 0; k < X_KEYS / 16; ++k)
             mma_f16_ts(tmem + X_O_COL, tmem + buf * X_S_COLS + 8 * k, v_desc + 128 * k, idesc_pv, (j | k) != 0);
-          if (!FP8) tc_commit(v_empty(st));
+          tc_commit(FP8 ? v16_empty((J + j) % C::V16S) : v_empty(st));
           if (j == tiles - 1) tc_commit(o_full);
         }
         if (j + 2 < tiles) issue_qk(j + 2);
@@ -414,14 +394,48 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       }
       const uint32_t x_ref = smem + C::X_AT + r * 4;
       auto x_group = [&](int g) { return x_ref + (1 + 2 * g) * X_ROWS * 4; };
+      const float shift = !FP8 ? 0.f : pass ? X_SHIFT_AGAIN : X_SHIFT_F16;
       float top = -INFINITY, l = 0.f;
       bool met = false;
       for (int j = (J + grp) & 1; j < tiles; j += 2) {
         const int tile = J + j;
+        const int st = tile % ST, key0 = (tile0 + j) * X_KEYS;
+        if (FP8) {
+          // This tile of V to bf16, while its scores are computed: a thread takes half a row, neighbours' stores in different
+          // banks.  Rows behind the last key become zeros, whatever the cache holds there: 0 . V has to be 0.
+          const int buf = tile % C::V16S;
+          ok = ok && mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD) &&
+               mbar_wait_warp(v16_empty(buf), ((tile / C::V16S) & 1) ^ 1, p.status, WK_ERR_TIMEOUT_MMA);
+          if (!ok) break;
+          constexpr int HALF = DH / 32;  // 16-byte pieces of half a row
+          const int row = r >> 1;
+          const uint32_t src = smem + C::V_AT + st * C::K_BYTES + row * 128;
+          const uint32_t dst = smem + C::V16_AT + buf * C::V16_BYTES + row * 128;
+          const bool behind = key0 + row >= keys;
+#pragma unroll
+          for (int c = 0; c < HALF; ++c) {
+            const int piece = (r & 1) * HALF + (HALF == 4 ? c ^ 2 * (r & 1) : c);
+            uint32_t w[4], o[8];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(src + ((piece ^ (row & 7)) << 4)));
+            if (behind) w[0] = w[1] = w[2] = w[3] = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              o[2 * x] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x]));
+              o[2 * x + 1] = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x] >> 16));
+            }
+            const uint32_t to = dst + (piece >> 2) * C::KV_SPAN;
+            const int at = (2 * piece) & 7;
+            sts128(to + ((at ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+            sts128(to + (((at + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
+          }
+          mbar_arrive(v_empty(st));
+          fence_proxy_async_smem();
+        }
         ok = ok && mbar_wait_warp(s_full(grp), (tile >> 1) & 1, p.status, WK_ERR_TIMEOUT_MMA);
         if (!ok) break;
         tc_fence_after();
-        const int key0 = (tile0 + j) * X_KEYS;
         const bool masked = __any_sync(0xffffffffu, key0 + X_KEYS - 1 > limit);
         const int last = limit - key0;  // columns beyond it are masked
         if (j == 0 && pass == 0) {
@@ -448,39 +462,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           met = true;
           if (j != 0 && pass == 0) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(m_ref) : "r"(x_ref) : "memory");
         }
-        const int st = tile % ST;
-        if (FP8) {
-          // this tile of V to bf16: a thread takes half a row.  Rows behind the last key become zeros, whatever the cache
-          // holds there: 0 . V has to be 0.
-          ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-          if (!ok) break;
-          constexpr int HALF = DH / 32;  // 16-byte pieces of half a row
-          const int row = r >> 1;
-          const uint32_t src = smem + C::V_AT + st * C::K_BYTES + row * 128;
-          const uint32_t dst = smem + C::V16_AT + grp * C::V16_BYTES + row * 128;
-          const bool behind = key0 + row >= keys;
-#pragma unroll
-          for (int c = 0; c < HALF; ++c) {
-            const int piece = (r & 1) * HALF + c;
-            uint32_t w[4], o[8];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(src + ((piece ^ (row & 7)) << 4)));
-            if (behind) w[0] = w[1] = w[2] = w[3] = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) e4m3x4_to_bf16(w[x], o[2 * x], o[2 * x + 1]);
-            if (e4m3x4_nan(w[0]) | e4m3x4_nan(w[1]) | e4m3x4_nan(w[2]) | e4m3x4_nan(w[3])) {
-#pragma unroll
-              for (int x = 0; x < 4; ++x) restore_nan(w[x], o[2 * x], o[2 * x + 1]);
-            }
-            const uint32_t to = dst + (piece >> 2) * C::KV_SPAN;
-            const int at = (2 * piece) & 7;
-            sts128(to + ((at ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
-            sts128(to + (((at + 1) ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
-          }
-          mbar_arrive(v_empty(st));
-          fence_proxy_async_smem();
-        } else if (key0 + X_KEYS > keys) {
+        if (!FP8 && key0 + X_KEYS > keys) {
           ok = mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
           if (!ok) break;
           const int row = r >> 1;
@@ -503,10 +485,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 if (c * 32 + i > last) raw[i] = 0xff800000u;
             }
             top = fmaxf(top, block_max(raw) * beta);
-            const float bias = m_ref > -INFINITY ? -m_ref : 0.f;
+            const float bias = m_ref > -INFINITY ? shift - m_ref : 0.f;
             uint32_t w[16];
             float sum;
-            softmax_block(raw, beta, bias, w, sum);
+            softmax_block<FP8>(raw, beta, bias, w, sum);
             l += sum;
             uint32_t lo[8], hi[8];
 #pragma unroll
@@ -532,9 +514,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(top2) : "r"(x_group(grp ^ 1) + X_ROWS * 4) : "memory");
       l += l2;
       top = fmaxf(top, top2);
-      far = ok && live && pass == 0 && top - m_ref > X_MAX_EXP;
+      far = ok && live && pass == 0 && top - m_ref > (FP8 ? X_MAX_EXP_F16 : X_MAX_EXP);
       inv_row = l > 0.f ? v_scale / l : l == l ? 0.f : l;  // NaN stays
-      lse_row = l == 0.f ? -INFINITY : m_ref + log2f(l);
+      lse_row = l == 0.f ? -INFINITY : m_ref - shift + log2f(l);
       if (pass == 0) m_ref = top;  // for the second pass
       tc_fence_after();
     }
@@ -801,14 +783,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <bool F16>
-__device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) {
-  if (!F16) return pack_bf16x2(lo, hi);
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // NT: groups of eight rows, 1 or 2.
 template <bool FP8, int DH, int NT>
 __global__ void __maxnreg__(NT == 1 ? 112 : 168)

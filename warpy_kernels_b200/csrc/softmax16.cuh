@@ -5,7 +5,16 @@
 
 namespace wk {
 
-// One block of 32 keys of one row: P as 16 bf16 pairs and the sum of the unrounded values.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) {
+  if (!F16) return pack_bf16x2(lo, hi);
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// One block of 32 keys of one row: P as 16 pairs of bf16 (or f16) and the sum of the unrounded values.
+template <bool F16 = false>
 __device__ __forceinline__ void softmax_block(const uint32_t (&sraw)[32], float beta, float bias, uint32_t (&w)[16],
                                               float& sum_exact) {
   const uint64_t beta2 = pack_f32x2(beta, beta), bias2 = pack_f32x2(bias, bias);
@@ -23,8 +32,8 @@ __device__ __forceinline__ void softmax_block(const uint32_t (&sraw)[32], float 
     p3 = ex2_approx(p3);
     acc01 = add_f32x2(acc01, pack_f32x2(p0, p1));
     acc23 = add_f32x2(acc23, pack_f32x2(p2, p3));
-    w[2 * i] = pack_bf16x2(p0, p1);
-    w[2 * i + 1] = pack_bf16x2(p2, p3);
+    w[2 * i] = pack_16x2<F16>(p0, p1);
+    w[2 * i + 1] = pack_16x2<F16>(p2, p3);
   }
   {
     float a0, a1, a2, a3;
