@@ -143,12 +143,6 @@ struct RowTarget {
   int64_t lse_to;
   int parts;
 };
-struct RowWeights {
-  float own[OWN_PARTS];     // of the parts of own keys
-  float member[X_CLUSTER];  // and of the cluster's
-  float inv;                // 1 / their sum
-};
-
 template <bool FP8, int DH>
 struct PrefixCfg {
   static constexpr int SIZE = FP8 ? 1 : 2;
@@ -173,7 +167,7 @@ struct PrefixCfg {
   static constexpr int SMEM = BAR_AT + 8 * (4 * STAGES + 7 + V16S) + 1024;
   // the exchange of a cluster takes the place of the tiles
   static constexpr int PART_BYTES = X_ROWS * (DH + X_PAD) * 4;
-  static_assert(PART_BYTES + X_ROWS * static_cast<int>(sizeof(RowWeights)) <= X_AT, "");
+  static_assert(PART_BYTES <= X_AT, "");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -282,7 +276,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
       targets[i] = e;
     }
   };
-  if (tiles == 0 && warp == 0) find_targets();
+  if (tiles == 0) {
+    if (warp == 0) find_targets();
+    __syncthreads();
+  }
 
   bool ok = true;  // no wait of this thread's role has given up
   float lse_row = -INFINITY, inv_row = 0.f;  // softmax threads: of their row, what its O is multiplied with
@@ -549,92 +546,110 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (grp == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + C::X_AT + r * 4), "f"(lse_row) : "memory");
     tc_fence_before();
   }
+  // ---- this CTA's rows, a warp to a row: what each of their parts counts, then the sums.  The parts of own keys are read
+  // ahead of their use, the first ones while the cluster meets.
+  constexpr int COLS = DH / 32, WARPS = X_THREADS / 32, AHEAD = 8;
+  static_assert(OWN_PARTS <= 32 && X_CLUSTER <= 32, "a lane for each of a row's parts");
+  float own_lse = -INFINITY, ahead[AHEAD][COLS];
+  auto read_own = [&](const RowTarget& e, int k0) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+#pragma unroll
+      for (int x = 0; x < COLS; ++x) ahead[k][x] = 0.f;
+      if (k0 + k >= e.parts) continue;
+      const float* src = p.part + (e.first + (k0 + k) * p.own_slot) * DH + lane * COLS;
+      if (COLS == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+        ahead[k][0] = v.x, ahead[k][1] = v.y, ahead[k][COLS - 2] = v.z, ahead[k][COLS - 1] = v.w;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+        ahead[k][0] = v.x, ahead[k][1] = v.y;
+      }
+    }
+  };
+  auto begin = [&](int i) {
+    if (OWN || i >= mine) return;
+    const RowTarget& e = targets[i];
+    own_lse = lane < e.parts ? __ldcg(p.part_lse + e.first + lane * p.own_slot) : -INFINITY;
+    read_own(e, 0);
+  };
   const bool meet = !OWN && p.cluster > 1;
-  if (meet) cluster_sync();
+  __syncwarp();
+  if (meet) cluster_arrive();
+  if (beside) pdl_wait();  // nothing that comes after this kernel starts before the one for own keys has ended
+  begin(warp);
+  __syncwarp();
+  if (meet) cluster_wait();
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, X_TMEM_COLS);
   }
-
-  // ---- this CTA's rows: what each of their parts counts, one thread to a row, then the sums
-  if (beside) pdl_wait();  // nothing that comes after this kernel starts before the one for own keys has ended
-  RowWeights* weights = reinterpret_cast<RowWeights*>(part + C::PART_BYTES);
-  if (final && beside) {
-    for (int i = threadIdx.x; i < mine * OWN_PARTS; i += X_THREADS) {
-      const RowTarget& e = targets[i / OWN_PARTS];
-      const int k = i % OWN_PARTS;
-      if (k < e.parts) weights[i / OWN_PARTS].own[k] = __ldcg(p.part_lse + e.first + k * p.own_slot);
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x < mine) {
-    const RowTarget& at = targets[threadIdx.x];
-    RowWeights& e = weights[threadIdx.x];
-    const uint32_t stat = smem + C::X_AT + (threadIdx.x * members + rank) * 4;
-    float lse[X_CLUSTER], top = -INFINITY, total = 0.f;
+  for (int i = warp; i < mine; i += WARPS) {
+    const RowTarget e = targets[i];
+    const int r = i * members + rank;
+    const uint32_t stat = smem + C::X_AT + r * 4, at = smem + (r * (DH + X_PAD) + lane * COLS) * 4;
+    float lse = -INFINITY;
+    if (lane < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(lse) : "r"(meet ? mapa(stat, lane) : stat));
+    float top = fmaxf(own_lse, lse);
 #pragma unroll
-    for (int k = 0; k < X_CLUSTER; ++k) {
-      lse[k] = -INFINITY;
-      if (k < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(lse[k]) : "r"(meet ? mapa(stat, k) : stat));
-    }
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float w_own = own_lse == -INFINITY ? 0.f : exp2f(own_lse - top), w = lse == -INFINITY ? 0.f : exp2f(lse - top);
+    float total = w_own + w;
 #pragma unroll
-    for (int k = 0; k < X_CLUSTER; ++k) top = fmaxf(top, lse[k]);
-    for (int k = 0; k < at.parts; ++k) top = fmaxf(top, e.own[k]);
-    for (int k = 0; k < at.parts; ++k) {
-      e.own[k] = e.own[k] == -INFINITY ? 0.f : exp2f(e.own[k] - top);
-      total += e.own[k];
-    }
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    float o[COLS];
 #pragma unroll
-    for (int k = 0; k < X_CLUSTER; ++k) {
-      e.member[k] = lse[k] == -INFINITY ? 0.f : exp2f(lse[k] - top);
-      total += e.member[k];
+    for (int x = 0; x < COLS; ++x) o[x] = 0.f;
+    for (int k0 = 0; !OWN && k0 < e.parts; k0 += AHEAD) {
+      if (k0) read_own(e, k0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float f = __shfl_sync(0xffffffffu, w_own, k0 + k);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) o[x] = fmaf(ahead[k][x], f, o[x]);
+      }
+    }
+    begin(i + WARPS);
+    for (int k0 = 0; k0 < members; k0 += AHEAD) {
+      float v[AHEAD][COLS];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) v[k][x] = 0.f;
+        if (k0 + k >= members) continue;
+        const uint32_t src = meet ? mapa(at, k0 + k) : at;
+        if (COLS == 4)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[k][0]), "=f"(v[k][1]), "=f"(v[k][COLS - 2]), "=f"(v[k][COLS - 1])
+                       : "r"(src));
+        else
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k][0]), "=f"(v[k][1]) : "r"(src));
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float f = __shfl_sync(0xffffffffu, w, k0 + k);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) o[x] = fmaf(v[k][x], f, o[x]);
+      }
     }
     const bool empty = total == 0.f;
-    e.inv = empty ? 0.f : 1.f / total;
-    const float y = empty ? INFINITY : top + log2f(total);
-    if (!final) p.part_lse[at.to] = empty ? -INFINITY : y;
-    else if (p.lse) p.lse[at.lse_to] = p.lse_natural ? y * 0.6931471805599453f : y;
-  }
-  __syncthreads();
-  constexpr int QUADS = DH / 4;
-  for (int i = threadIdx.x; i < mine * QUADS; i += X_THREADS) {
-    const int c = i % QUADS, r = i / QUADS * members + rank;
-    const RowTarget& e = targets[i / QUADS];
-    const RowWeights& w = weights[i / QUADS];
-    const uint32_t at = smem + r * (DH + X_PAD) * 4 + c * 16;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float f, const float4& v) {
-      o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-    };
-    for (int k0 = 0; k0 < e.parts; k0 += 8) {
-      float4 v[8];
+    const float inv = empty ? 0.f : 1.f / total, y = empty ? INFINITY : top + log2f(total);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + k < e.parts) v[k] = __ldcg(reinterpret_cast<const float4*>(p.part + (e.first + (k0 + k) * p.own_slot) * DH) + c);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) add(k0 + k < e.parts ? w.own[k0 + k] : 0.f, v[k]);
+    for (int x = 0; x < COLS; ++x) o[x] *= inv;
+    if (final) {
+      __nv_bfloat16* dst = p.out + e.to + lane * COLS;
+      if (COLS == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[COLS - 2], o[COLS - 1]));
+      else
+        *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0], o[1]);
+      if (p.lse && lane == 0) p.lse[e.lse_to] = p.lse_natural ? y * 0.6931471805599453f : y;
+    } else {
+      float* dst = p.part + e.to * DH + lane * COLS;
+      if (COLS == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[COLS - 2], o[COLS - 1]);
+      else *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
+      if (lane == 0) p.part_lse[e.to] = empty ? -INFINITY : y;
     }
-    for (int k0 = 0; k0 < members; k0 += 8) {
-      float4 v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + k < members)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
-                       : "r"(meet ? mapa(at, k0 + k) : at));
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) add(w.member[k0 + k], v[k]);
-    }
-    o.x *= w.inv, o.y *= w.inv, o.z *= w.inv, o.w *= w.inv;
-    if (final)
-      *reinterpret_cast<uint2*>(p.out + e.to + 4 * c) = make_uint2(pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w));
-    else
-      reinterpret_cast<float4*>(p.part + e.to * DH)[c] = o;
   }
   __syncwarp();
   if (meet) cluster_sync();  // nobody leaves while its part may still be read
