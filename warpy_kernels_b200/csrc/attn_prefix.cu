@@ -832,28 +832,29 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
   OwnWalker<FP8, DH> now(p, line, cum, lengths, blocks, piece), ahead = now;
   // Slots are filled in turn: K of a step, V of it, K of the next.
-  int fetched = 0;
-  auto fetch = [&](int by) {
+  int to = 0;
+  auto fetch = [&](bool is_v, int by) {
     if (!ahead.here()) return;
-    const int slot = fetched % C::SLOTS, is_v = fetched & 1;
     if (lane == by) {
-      const uint32_t dst = ring + slot * C::SLOT_BYTES, bar = bars + 8 * slot;
+      const uint32_t dst = ring + to * C::SLOT_BYTES, bar = bars + 8 * to;
       mbar_expect_tx(bar, C::SLOT_BYTES);
       for (int i = 0; i < C::SPANS; ++i)
         tma_load_4d(dst + i * C::SPAN_BYTES, is_v ? &map_v : &map_k, bar, 64 * i, ahead.step * C::KEYS, ahead.h, ahead.b);
     }
-    ++fetched;
+    to = to + 1 == C::SLOTS ? 0 : to + 1;
     if (is_v && ++ahead.step == ahead.end) ahead.next(p, blocks);
   };
-  for (int i = 0; i < C::SLOTS; ++i) fetch(0);
+#pragma unroll
+  for (int i = 0; i < C::SLOTS; ++i) fetch(i & 1, 0);
 
-  int used = 0;
+  int from = 0;
+  uint32_t parity = 0;
   bool ok = true;
   auto arrive_at = [&]() {  // the slot in turn, its data there
-    const int slot = used % C::SLOTS;
-    ok = ok && mbar_wait_warp(bars + 8 * slot, (used / C::SLOTS) & 1, p.status, WK_ERR_TIMEOUT_LOAD);
-    ++used;
-    return ring + slot * C::SLOT_BYTES;
+    const uint32_t at = ring + from * C::SLOT_BYTES;
+    ok = ok && mbar_wait_warp(bars + 8 * from, parity, p.status, WK_ERR_TIMEOUT_LOAD);
+    if (++from == C::SLOTS) from = 0, parity ^= 1;
+    return at;
   };
   for (; now.here(); now.next(p, blocks)) {
     const int row0 = now.block * Y_ROWS, sc = now.b * p.Hkv + now.h, unit = now.b * per_seq + now.u;
@@ -940,15 +941,14 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int n = 0; n < N16; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[i][n][j] *= beta;
+          for (int j = 0; j < 4; ++j)
             if (masked && key0 + 16 * n + g + 8 * (j >> 1) > limit[i][j & 1]) s[i][n][j] = -INFINITY;
-          }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           mx[i][j] = fmaxf(s[i][0][j], s[i][0][2 + j]);
 #pragma unroll
           for (int n = 1; n < N16; ++n) mx[i][j] = max3(mx[i][j], s[i][n][j], s[i][n][2 + j]);
+          mx[i][j] *= beta;
         }
       }
 #pragma unroll
@@ -961,7 +961,7 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
       for (int i = 0; i < NT; ++i) move |= mx[i][0] > m[i][0] + 1.f || mx[i][1] > m[i][1] + 1.f;
       move = __any_sync(0xffffffffu, move);
-      fetch(0);  // into K's place: by now every lane has its scores, so all of K has been read
+      fetch(C::SLOTS % 2, 0);  // into K's place: by now every lane has its scores, so all of K has been read
       if (move) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -986,7 +986,7 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
         for (int n = 0; n < N16; ++n) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][n][j] = ex2_approx(s[i][n][j] + bias[j & 1]);
+          for (int j = 0; j < 4; ++j) s[i][n][j] = ex2_approx(fmaf(s[i][n][j], beta, bias[j & 1]));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             l[i][j] += s[i][n][j] + s[i][n][2 + j];
@@ -1016,10 +1016,9 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             ldmatrix_x4_trans(w, vs + key * 128 + (((k + lane / 8 % 2) ^ (key & 7)) << 4));
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // 16 elements: pair g of the codes becomes rows g and g + 8
-              const uint32_t y0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x])), y1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[x] >> 16));
-              const uint32_t z0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 + x])), z1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w[2 + x] >> 16));
-              const uint32_t a0 = __byte_perm(y0, y1, 0x5410), a1 = __byte_perm(y0, y1, 0x7632);
-              const uint32_t a2 = __byte_perm(z0, z1, 0x5410), a3 = __byte_perm(z0, z1, 0x7632);
+              const uint32_t y = __byte_perm(w[x], 0, 0x3120), z = __byte_perm(w[2 + x], 0, 0x3120);
+              const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(y)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(y >> 16));
+              const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(z)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(z >> 16));
 #pragma unroll
               for (int i = 0; i < NT; ++i) mma_16816<true>(o[i][k + x], a0, a1, a2, a3, pt[i][n][0], pt[i][n][1]);
             }
@@ -1037,7 +1036,7 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       }
       // Into V's place, which every lane has read once it has a sum that its last fragment went into.  The vote waits for
       // that; which lane then issues the load is all the same.
-      fetch(__any_sync(0xffffffffu, o[NT - 1][C::K16 - 1][0] == -1.23456789e-30f) ? 1 : 0);
+      fetch(C::SLOTS % 2 == 0, __any_sync(0xffffffffu, o[NT - 1][C::K16 - 1][0] == -1.23456789e-30f) ? 1 : 0);
     }
 
     // ---- this warp's part: O / l and the log-sum-exp
