@@ -105,6 +105,20 @@ def test_against_float64(cuda, B, Hq, Hkv, Nq, P, S, d, fp8, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B, Hq, Hkv, Nq, P, S, d", [
+    (20, 16, 8, 5, 100, 520, 128), (20, 16, 8, 5, 0, 511, 64), (50, 12, 4, 6, 70, 90, 64), (38, 4, 4, 31, 130, 65, 128)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_sequences_that_fill_the_gpu(cuda, B, Hq, Hkv, Nq, P, S, d, fp8):
+    """Nine rows a sequence and more, where which kernel takes own keys depends on how many and how long they are."""
+    t = make(B, Hq, Hkv, Nq, P, S, d, fp8)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    used = torch.randint(0, S + 1, (B,), device="cuda", generator=g, dtype=torch.int32)
+    used[:2] = torch.tensor([0, S], device="cuda", dtype=torch.int32)
+    for causal in (False, True):
+        check(t, wk.attn_fwd_shared_prefix(**t, causal=causal, seqused_k=used), causal, used)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [False, True])
 def test_lengths_of_zero(cuda, fp8):
     for P, S in ((0, 100), (100, 0), (0, 0), (0, 1), (1, 0)):

@@ -7,8 +7,8 @@
 // head are stacked, 128 to a tile, and go over the prefix together; the rows of one sequence (its group of query heads
 // times its queries) go over its own keys.
 //
-// Own keys come first, and leave parts: O / l and the log-sum-exp of every row, fp32.  Up to 32 rows a sequence, that is a
-// kernel on mma.sync whose warps work by themselves; more rows take the tensor-core kernel below, one CTA for 128 of them.
+// Own keys come first, and leave parts: O / l and the log-sum-exp of every row, fp32.  Few rows a sequence take a kernel on
+// mma.sync whose warps work by themselves, more the tensor-core kernel below, one CTA for 128 of them (own_by_rows).
 // The prefix: a unit is 128 stacked rows, and S = Q.K^T and O += P.V go by 128 x 64 tiles on tcgen05.  A unit's tiles are
 // divided over the CTAs of a cluster, which meet in distributed shared memory, add the own keys' parts and write the output.
 // Where units are few, several clusters share one; then they leave parts too, and a last kernel adds up all of them.  The
@@ -16,13 +16,24 @@
 //
 // One CTA of the tensor-core kernel (two per SM, 320 threads): warp 0 TMA producer, warp 1 issues the products, two softmax
 // groups of four warps take the tiles in turn, one thread per row: the structure of attn_fwd_bf16.cu.  P is bf16 and
-// overwrites its scores in tensor memory.  FP8: scores from e4m3 (kind::f8f6f4); V tiles are converted to bf16 (exact) in
-// shared memory by the group that has the tile, so that P keeps 8 bits.
+// overwrites its scores in tensor memory.  FP8: scores from e4m3 (kind::f8f6f4); V tiles become f16 (exact) in shared memory,
+// by the group that has the tile and while its scores are computed, and P is f16.
 //
-// Numerics: logits in base 2.  Tensor-core kernel: the row reference is the maximum of the CTA's first tile (bf16 has the
-// exponent range to leave it there); a CTA in which a row rises more than 2^60 above it goes through its keys once more, with
-// the maxima it then knows.  Kernel for few rows: the reference moves when a score exceeds it by more than 1; P is bf16, or
-// f16 times 2^14 for FP8 inputs, whose K and V become f16 (exact).
+// Numerics: logits in base 2; statistics, sums and parts in fp32.  P is rounded to 16 bits for the tensor core: by 2^-8 of
+// itself in bf16, 2^-11 in f16; the row sums take it before that.  Tensor-core kernel: the row reference is the maximum of
+// the CTA's first tile; a CTA in which a row rises more than 2^60 above it (bf16 has the exponent range) goes through its
+// keys once more, with the maxima it then knows.  FP8: f16 P is stored times 2^5 and may rise 2^10; one below 2^-19 of the
+// reference is off by 2^-30 of it at most.  Kernel for few rows: the reference moves when a score exceeds it by more than 1;
+// P is bf16, or f16 times 2^14 for FP8 inputs, whose K and V become f16 (exact).
+//
+// What bounds it.  The prefix kernel: 1090 cycles per 128 x 64 tile and SM, where the exponentials need 512 and the products
+// 400 to 640 (ncu: MUFU 50 %, tensor pipe 37 %, issue slots 52 %): the chain scores -> P -> product with two groups in each
+// of two CTAs.  128 rows of 8 heads over 32768 keys 130 us FP8, 135 us bf16 (530 / 510 TFLOP/s).  (V to bf16 by integer
+// arithmetic instead, behind the scores: 164 us; 128-key tiles in one CTA per SM, tensor memory read ahead, waits that poll: no
+// faster.)  Own keys: their bytes in bf16 (97 us for 537 MB), the latency of a warp's instructions in FP8 (64 us for 268 MB).
+// Whole calls, inputs from HBM: 16 sequences, 64 / 8 heads, 8192 shared and up to 1024 own bf16 keys 26.5 us; 128 sequences,
+// 32768 and up to 2048 FP8 keys 200 to 210 us; 24 sequences, 32 / 8 heads, 5 queries, 4096 and up to 512 bf16 keys 36 us;
+// 64 sequences, 32 heads, 2048 and up to 300 FP8 keys 33.5 us.
 #include <math.h>
 
 #include "common.cuh"
@@ -49,7 +60,6 @@ constexpr int X_PAD = 4;       // values between rows in the exchange: lanes wit
 constexpr int Y_START = 1;  // what a unit of the kernel for few rows weighs beside its steps
 constexpr int Y_WARPS = 4;
 constexpr int Y_ROWS = 16;      // rows of one of its units, at most
-constexpr int Y_FEW_ROWS = 32;  // rows of a sequence up to which that kernel takes them
 constexpr int Y_CUM = 1024;     // sequences whose weights are summed in shared memory
 constexpr int OWN_PARTS = 32;   // parts of a unit of own keys, at most
 
@@ -667,8 +677,10 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
 // movmatrix.  FP8: ldmatrix moves pairs of codes; which index of the head dimension a pair stands for is the same for K and
 // Q, and only moves O's rows for V.
 //
-// Bound by reading K and V once; with eight warps on an SM their latency is what shows.  About 110 instructions for 16
-// keys (FP8: 340 for 32).
+// Bound by reading K and V once in bf16; in FP8 by a warp's instructions, about 570 for 32 keys (134 of them conversions) at
+// one in five cycles, with eight warps on an SM.  (Sixteen warps with the SM to themselves, the prefix kernel behind them: 128
+// sequences, 32768 and 2048 keys 197 -> 191 us FP8, 239 -> 243 bf16; 16 sequences, 8192 and 1024 keys 28.5 -> 36.  The e4m3 form
+// of mma.sync: no fewer conversions.)
 
 // Exclusive sums of the sequences' weights, by the whole CTA, and their lengths; both in shared or global memory.
 template <int KEYS>
@@ -1146,6 +1158,19 @@ void divide_prefix(int sms, Sizes& z) {
     }
 }
 
+// Whether own keys go to the kernel for few rows, which divides them evenly over the SMs and runs beside the prefix kernel;
+// the tensor-core kernel takes a sequence's keys in one CTA and all its rows at once.  The latter wins with more than eight
+// rows (two of the former's column blocks; from 17 on it reads the keys twice, from 33 on three times) where sequences fill
+// the SMs and, up to 16 rows, are long enough for its start.  bf16, 4096 shared keys, own keys up to S, us of few rows and of
+// tiles:
+//    64 x 8 heads, S 1024: 12 rows 70, 63; 20 rows 121, 81; 32 rows 130, 88      24 x 8, S 512: 12 rows 34, 32; 32 rows 51, 42
+//   300 x 8 heads, S 200: 12 rows 145, 156; 20 rows 235, 212                      8 x 8, S 1024: 12 rows 22, 27; 32 rows 30, 31
+//     4 x 1 heads, S 8192: 20 rows 30, 96                              FP8, 64 x 8, S 1024: 12 rows 62, 57; 20 rows 98, 75
+bool own_by_rows(int64_t rows, int64_t sequences, int S, int sms) {
+  if (rows <= 8) return true;
+  return sequences <= sms ? rows <= 32 : rows <= 16 && S < 512;
+}
+
 // false if the problem is beyond the kernels' 32-bit counts.
 bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Sizes& z) {
   const int64_t rows_own = static_cast<int64_t>(Hq / Hkv) * Nq, rows_all = rows_own * B;
@@ -1156,7 +1181,7 @@ bool sizes_of(int B, int Hq, int Hkv, int Nq, int P, int S, int d, int sms, Size
   z.units_p = z.tiles_p ? Hkv * z.blocks_p : 0;
   z.cluster = z.splits = 1;
   if (z.units_p) divide_prefix(sms, z);
-  z.by_rows = rows_own <= Y_FEW_ROWS;
+  z.by_rows = own_by_rows(rows_own, static_cast<int64_t>(B) * Hkv, S, sms);
   const int unit_rows = z.by_rows ? Y_ROWS : X_ROWS;
   z.own_slot = rows_own < unit_rows ? z.rows_own : unit_rows;
   z.blocks_own = static_cast<int>((rows_own + unit_rows - 1) / unit_rows);
@@ -1197,7 +1222,7 @@ int launch_prefix(const CUtensorMap (&maps)[4], const Sizes& z, PrefixParams& p,
       return bad;
   } else if (z.units_own) {
     const void* fn = reinterpret_cast<const void*>(attn_prefix_kernel<FP8, DH, true>);
-    if (allow_smem(fn, C::SMEM)) return WK_E_CUDA;
+    if (allow_smem(fn, C::SMEM) || prefer_smem(fn)) return WK_E_CUDA;
     if (int bad = launch_pdl(fn, dim3(z.units_own), X_THREADS, C::SMEM, stream, 1,
                              {const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]), &p}))
       return bad;

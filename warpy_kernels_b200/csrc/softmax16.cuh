@@ -1,4 +1,4 @@
-// Softmax of one row's scores as the kernels with bf16 probabilities take them out of tensor memory: blocks of 32 keys in
+// Softmax of one row's scores as the kernels with 16-bit probabilities take them out of tensor memory: blocks of 32 keys in
 // one thread.
 #pragma once
 #include "common.cuh"
