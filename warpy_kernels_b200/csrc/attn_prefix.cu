@@ -32,7 +32,7 @@
 // arithmetic instead, behind the scores: 164 us; 128-key tiles in one CTA per SM, tensor memory read ahead, waits that poll: no
 // faster.)  Own keys: their bytes in bf16 (97 us for 537 MB), the latency of a warp's instructions in FP8 (64 us for 268 MB).
 // Whole calls, inputs from HBM: 16 sequences, 64 / 8 heads, 8192 shared and up to 1024 own bf16 keys 26.5 us; 128 sequences,
-// 32768 and up to 2048 FP8 keys 200 to 210 us; 24 sequences, 32 / 8 heads, 5 queries, 4096 and up to 512 bf16 keys 36 us;
+// 32768 and up to 2048 FP8 keys 200 to 210 us; 24 sequences, 32 / 8 heads, 5 queries, 4096 and up to 512 bf16 keys 38 us;
 // 64 sequences, 32 heads, 2048 and up to 300 FP8 keys 33.5 us.
 #include <math.h>
 
