@@ -36,6 +36,8 @@
 // 64 sequences, 32 heads, 2048 and up to 300 FP8 keys 33.5 us.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_common.h"
 #include "pair.cuh"
@@ -260,9 +262,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     tile0 = 0, tiles = (keys + X_KEYS - 1) / X_KEYS;
   }
 
-  const int rank = OWN ? 0 : blockIdx.x % p.cluster, members = OWN ? 1 : p.cluster;
+  const int rank = blockIdx.x % p.cluster, members = p.cluster;
   const int mine = rank < rows ? (rows - rank + members - 1) / members : 0;  // the rows congruent to this CTA's rank
-  const bool final = !OWN && p.splits == 1;
+  const bool final = p.splits == 1;
   uint8_t* smem_ptr = smem_raw + (smem - smem_u32(smem_raw));
   RowTarget* targets = reinterpret_cast<RowTarget*>(smem_ptr + C::TARGET_AT);
   auto find_targets = [&]() {  // by the producer warp
@@ -270,8 +272,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     for (int i = lane; i < mine; i += 32) {
       const int r = i * members + rank;
       RowTarget e = {};
-      int seq = b, own = row0 + r;
-      if (!OWN) seq = own / p.rows_own, own -= seq * p.rows_own;
+      int own = row0 + r;
+      const int seq = own / p.rows_own;
+      own -= seq * p.rows_own;
       if (final) {
         const int g = own / p.Nq, n = own - g * p.Nq, head = h * p.group + g;
         e.to = seq * p.out_strides[0] + head * p.out_strides[1] + n * p.out_strides[2];
@@ -281,15 +284,11 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           e.first = parts.first, e.parts = parts.count;
         }
       } else {
-        e.to = OWN ? own_slot_of(p, blockIdx.x, 0) + r : static_cast<int64_t>(blockIdx.x / p.cluster) * X_ROWS + r;
+        e.to = static_cast<int64_t>(blockIdx.x / p.cluster) * X_ROWS + r;
       }
       targets[i] = e;
     }
   };
-  if (tiles == 0) {
-    if (warp == 0) find_targets();
-    __syncthreads();
-  }
 
   bool ok = true;  // no wait of this thread's role has given up
   float lse_row = -INFINITY, inv_row = 0.f;  // softmax threads: of their row, what its O is multiplied with
@@ -317,7 +316,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         }
       }
       __syncwarp();
-      if (pass == 0) find_targets();
+      if (!OWN && pass == 0) find_targets();
     } else if (warp == 1) {
       const bool mine = elect_one();
       constexpr uint32_t idesc_qk = FP8 ? make_idesc(0, 0, 0, 0, X_ROWS, X_KEYS) : make_idesc(1, 1, 0, 0, X_ROWS, X_KEYS);
@@ -530,7 +529,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     if (!__syncthreads_or(far) || pass) break;
   }
 
-  // ---- this CTA's part to shared memory: every tile and product has been used
+  // ---- this CTA's part: every tile and product has been used.  Own keys' goes to memory, the prefix's to shared memory.
+  const int64_t own_slot = OWN ? own_slot_of(p, blockIdx.x, 0) : 0;
   uint8_t* part = smem_ptr;  // [row][DH + X_PAD]
   if (warp >= 2) {
     const int quad = warp & 3, grp = (warp - 2) >> 2, r = quad * 32 + lane;
@@ -547,120 +547,172 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
           for (int i = 0; i < 32; ++i) v[i] = 0;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          reinterpret_cast<float4*>(part + r * (DH + X_PAD) * 4)[grp * (DH / 8) + c * 8 + i] =
-              make_float4(__uint_as_float(v[4 * i]) * inv_row, __uint_as_float(v[4 * i + 1]) * inv_row,
-                          __uint_as_float(v[4 * i + 2]) * inv_row, __uint_as_float(v[4 * i + 3]) * inv_row);
+        for (int i = 0; i < 8; ++i) {
+          const int at = grp * (DH / 8) + c * 8 + i;
+          const float4 y = make_float4(__uint_as_float(v[4 * i]) * inv_row, __uint_as_float(v[4 * i + 1]) * inv_row,
+                                       __uint_as_float(v[4 * i + 2]) * inv_row, __uint_as_float(v[4 * i + 3]) * inv_row);
+          if (!OWN) reinterpret_cast<float4*>(part + r * (DH + X_PAD) * 4)[at] = y;
+          else if (r < rows) reinterpret_cast<float4*>(p.part + (own_slot + r) * DH)[at] = y;
+        }
       }
     }
-    if (grp == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + C::X_AT + r * 4), "f"(lse_row) : "memory");
+    if (OWN && grp == 0 && r < rows) p.part_lse[own_slot + r] = lse_row;
+    if (!OWN && grp == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem + C::X_AT + r * 4), "f"(lse_row) : "memory");
     tc_fence_before();
   }
-  // ---- this CTA's rows, a warp to a row: what each of their parts counts, then the sums.  The parts of own keys are read
-  // ahead of their use, the first ones while the cluster meets.
-  constexpr int COLS = DH / 32, WARPS = X_THREADS / 32, AHEAD = 8;
+  if (OWN) {
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, X_TMEM_COLS);
+    }
+    return;
+  }
+
+  // ---- this CTA's rows, one or several to a warp at a time: what each of their parts counts, then the sums.  The parts of
+  // own keys are read ahead of their use, the first ones while the cluster meets.
+  constexpr int COLS = DH / 32, WARPS = X_THREADS / 32;
   static_assert(OWN_PARTS <= 32 && X_CLUSTER <= 32, "a lane for each of a row's parts");
-  float own_lse = -INFINITY, ahead[AHEAD][COLS];
-  auto read_own = [&](const RowTarget& e, int k0) {
+  const bool meet = p.cluster > 1;
+  auto join = [&](auto rows_at_once, auto parts_at_once) {
+    constexpr int ROWS = decltype(rows_at_once)::value, AHEAD = decltype(parts_at_once)::value;
+    float own_lse[ROWS], ahead[ROWS][AHEAD][COLS];
+    auto read_own = [&](const RowTarget& e, int k0, float (&to)[AHEAD][COLS]) {
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
+      for (int k = 0; k < AHEAD; ++k) {
 #pragma unroll
-      for (int x = 0; x < COLS; ++x) ahead[k][x] = 0.f;
-      if (k0 + k >= e.parts) continue;
-      const float* src = p.part + (e.first + (k0 + k) * p.own_slot) * DH + lane * COLS;
-      if (COLS == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-        ahead[k][0] = v.x, ahead[k][1] = v.y, ahead[k][COLS - 2] = v.z, ahead[k][COLS - 1] = v.w;
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-        ahead[k][0] = v.x, ahead[k][1] = v.y;
+        for (int x = 0; x < COLS; ++x) to[k][x] = 0.f;
+        if (k0 + k >= e.parts) continue;
+        const float* src = p.part + (e.first + (k0 + k) * p.own_slot) * DH + lane * COLS;
+        if (COLS == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          to[k][0] = v.x, to[k][1] = v.y, to[k][COLS - 2] = v.z, to[k][COLS - 1] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          to[k][0] = v.x, to[k][1] = v.y;
+        }
+      }
+    };
+    auto begin = [&](int i0) {
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+        const int i = i0 + q * WARPS;
+        own_lse[q] = -INFINITY;
+        if (i >= mine) continue;
+        const RowTarget& e = targets[i];
+        if (lane < e.parts) own_lse[q] = __ldcg(p.part_lse + e.first + lane * p.own_slot);
+        read_own(e, 0, ahead[q]);
+      }
+    };
+    __syncwarp();
+    if (meet) cluster_arrive();
+    if (beside) pdl_wait();  // nothing that comes after this kernel starts before the one for own keys has ended
+    begin(warp);
+    __syncwarp();
+    if (meet) cluster_wait();
+    else __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, X_TMEM_COLS);
+    }
+    for (int i0 = warp; i0 < mine; i0 += ROWS * WARPS) {
+      float top[ROWS], w_own[ROWS], w[ROWS], total[ROWS], o[ROWS][COLS];
+      uint32_t at[ROWS];
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+        const int r = min(i0 + q * WARPS, mine - 1) * members + rank;
+        const uint32_t stat = smem + C::X_AT + r * 4;
+        at[q] = smem + (r * (DH + X_PAD) + lane * COLS) * 4;
+        w[q] = -INFINITY;
+        if (lane < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w[q]) : "r"(meet ? mapa(stat, lane) : stat));
+        top[q] = fmaxf(own_lse[q], w[q]);
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1)
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) top[q] = fmaxf(top[q], __shfl_xor_sync(0xffffffffu, top[q], x));
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+        w_own[q] = own_lse[q] == -INFINITY ? 0.f : exp2f(own_lse[q] - top[q]);
+        w[q] = w[q] == -INFINITY ? 0.f : exp2f(w[q] - top[q]);
+        total[q] = w_own[q] + w[q];
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1)
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) total[q] += __shfl_xor_sync(0xffffffffu, total[q], x);
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) o[q][x] = 0.f;
+        if (i0 + q * WARPS >= mine) continue;
+        const RowTarget& e = targets[i0 + q * WARPS];
+        for (int k0 = 0; k0 < e.parts; k0 += AHEAD) {
+          if (k0) read_own(e, k0, ahead[q]);
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const float f = __shfl_sync(0xffffffffu, w_own[q], k0 + k);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) o[q][x] = fmaf(ahead[q][k][x], f, o[q][x]);
+          }
+        }
+      }
+      begin(i0 + ROWS * WARPS);
+      for (int k0 = 0; k0 < members; k0 += AHEAD) {
+        float v[ROWS][AHEAD][COLS];
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) v[q][k][x] = 0.f;
+            if (k0 + k >= members) continue;
+            const uint32_t src = meet ? mapa(at[q], k0 + k) : at[q];
+            if (COLS == 4)
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(v[q][k][0]), "=f"(v[q][k][1]), "=f"(v[q][k][COLS - 2]), "=f"(v[q][k][COLS - 1])
+                           : "r"(src));
+            else
+              asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[q][k][0]), "=f"(v[q][k][1]) : "r"(src));
+          }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+          for (int q = 0; q < ROWS; ++q) {
+            const float f = __shfl_sync(0xffffffffu, w[q], k0 + k);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) o[q][x] = fmaf(v[q][k][x], f, o[q][x]);
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) {
+        if (i0 + q * WARPS >= mine) continue;
+        const RowTarget& e = targets[i0 + q * WARPS];
+        const bool empty = total[q] == 0.f;
+        const float inv = empty ? 0.f : 1.f / total[q], y = empty ? INFINITY : top[q] + log2f(total[q]);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) o[q][x] *= inv;
+        if (final) {
+          __nv_bfloat16* dst = p.out + e.to + lane * COLS;
+          if (COLS == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[q][0], o[q][1]), pack_bf16x2(o[q][COLS - 2], o[q][COLS - 1]));
+          else
+            *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[q][0], o[q][1]);
+          if (p.lse && lane == 0) p.lse[e.lse_to] = p.lse_natural ? y * 0.6931471805599453f : y;
+        } else {
+          float* dst = p.part + e.to * DH + lane * COLS;
+          if (COLS == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[q][0], o[q][1], o[q][COLS - 2], o[q][COLS - 1]);
+          else *reinterpret_cast<float2*>(dst) = make_float2(o[q][0], o[q][1]);
+          if (lane == 0) p.part_lse[e.to] = empty ? -INFINITY : y;
+        }
       }
     }
   };
-  auto begin = [&](int i) {
-    if (OWN || i >= mine) return;
-    const RowTarget& e = targets[i];
-    own_lse = lane < e.parts ? __ldcg(p.part_lse + e.first + lane * p.own_slot) : -INFINITY;
-    read_own(e, 0);
-  };
-  const bool meet = !OWN && p.cluster > 1;
-  __syncwarp();
-  if (meet) cluster_arrive();
-  if (beside) pdl_wait();  // nothing that comes after this kernel starts before the one for own keys has ended
-  begin(warp);
-  __syncwarp();
-  if (meet) cluster_wait();
-  else __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, X_TMEM_COLS);
-  }
-  for (int i = warp; i < mine; i += WARPS) {
-    const RowTarget e = targets[i];
-    const int r = i * members + rank;
-    const uint32_t stat = smem + C::X_AT + r * 4, at = smem + (r * (DH + X_PAD) + lane * COLS) * 4;
-    float lse = -INFINITY;
-    if (lane < members) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(lse) : "r"(meet ? mapa(stat, lane) : stat));
-    float top = fmaxf(own_lse, lse);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float w_own = own_lse == -INFINITY ? 0.f : exp2f(own_lse - top), w = lse == -INFINITY ? 0.f : exp2f(lse - top);
-    float total = w_own + w;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    float o[COLS];
-#pragma unroll
-    for (int x = 0; x < COLS; ++x) o[x] = 0.f;
-    for (int k0 = 0; !OWN && k0 < e.parts; k0 += AHEAD) {
-      if (k0) read_own(e, k0);
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const float f = __shfl_sync(0xffffffffu, w_own, k0 + k);
-#pragma unroll
-        for (int x = 0; x < COLS; ++x) o[x] = fmaf(ahead[k][x], f, o[x]);
-      }
-    }
-    begin(i + WARPS);
-    for (int k0 = 0; k0 < members; k0 += AHEAD) {
-      float v[AHEAD][COLS];
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-#pragma unroll
-        for (int x = 0; x < COLS; ++x) v[k][x] = 0.f;
-        if (k0 + k >= members) continue;
-        const uint32_t src = meet ? mapa(at, k0 + k) : at;
-        if (COLS == 4)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(v[k][0]), "=f"(v[k][1]), "=f"(v[k][COLS - 2]), "=f"(v[k][COLS - 1])
-                       : "r"(src));
-        else
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k][0]), "=f"(v[k][1]) : "r"(src));
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const float f = __shfl_sync(0xffffffffu, w, k0 + k);
-#pragma unroll
-        for (int x = 0; x < COLS; ++x) o[x] = fmaf(v[k][x], f, o[x]);
-      }
-    }
-    const bool empty = total == 0.f;
-    const float inv = empty ? 0.f : 1.f / total, y = empty ? INFINITY : top + log2f(total);
-#pragma unroll
-    for (int x = 0; x < COLS; ++x) o[x] *= inv;
-    if (final) {
-      __nv_bfloat16* dst = p.out + e.to + lane * COLS;
-      if (COLS == 4)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[COLS - 2], o[COLS - 1]));
-      else
-        *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0], o[1]);
-      if (p.lse && lane == 0) p.lse[e.lse_to] = p.lse_natural ? y * 0.6931471805599453f : y;
-    } else {
-      float* dst = p.part + e.to * DH + lane * COLS;
-      if (COLS == 4) *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[COLS - 2], o[COLS - 1]);
-      else *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
-      if (lane == 0) p.part_lse[e.to] = empty ? -INFINITY : y;
-    }
-  }
+  // A CTA of a small cluster has many rows with few parts, one of a large cluster few with many.  Four rows at a time against
+  // one, us: 79 sequences, 32 / 8 heads, 17 queries, 71 + 54 FP8 keys (one member) 60, 75; 64 sequences of 32 heads, 2048 + 300
+  // FP8 keys (four members) 35, 33.5.
+  if (members <= 2) join(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+  else join(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
   __syncwarp();
   if (meet) cluster_sync();  // nobody leaves while its part may still be read
 }
