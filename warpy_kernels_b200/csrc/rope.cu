@@ -190,7 +190,9 @@ struct Place {
     tslot = slot / p.hb, hslot = slot - tslot * p.hb;
     active = tslot < p.tb;
     turned = in_row < p.rot / 16;
-    if (p.interleaved || !turned) {
+    // neighbouring lanes' pieces lie side by side, also where pairs are neighbours and either half would do (4 x 13020 tokens,
+    // 16 / 2 heads of 160, interleaved, gradient: 273 us with each lane's pieces side by side, 186 so)
+    if (!turned) {
       at_a = 16 * in_row, at_b = at_a + 8;
     } else {
       at_a = 8 * in_row, at_b = at_a + p.rot / 2;
@@ -218,7 +220,7 @@ struct Place {
 };
 
 // The lane's cosines and sines of its token.  The lanes of a token divide its pairs and exchange them in `table`
-// ([token of the warp][cos, sin][pair]).
+// ([token of the warp][cos, sin][pair], eight of a lane's in a row: those of both halves' elements, or four of each piece).
 template <typename T, int LPR>
 __device__ __forceinline__ void angles(const RopeParams& p, const Place<LPR>& at, bool live, int b, int n, float* table,
                                        float (&c)[8], float (&s)[8]) {
@@ -230,7 +232,8 @@ __device__ __forceinline__ void angles(const RopeParams& p, const Place<LPR>& at
       double turns[2];  // two at a time: their loads go together
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int j = min(j0 + i * every, pairs - 1);
+        const int place = min(j0 + i * every, pairs - 1);
+        const int j = p.interleaved ? (place >> 3) * 4 + (place & 3) + (place & 4 ? pairs / 2 : 0) : place;
         const int axis = static_cast<int>(p.axis_map[j >> 5] >> (2 * (j & 31))) & 3;
         const int64_t from = axis * p.ps[0] + b * p.ps[1] + n * p.ps[2];
         const double pos = p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[from])
