@@ -192,11 +192,8 @@ struct Place {
     turned = in_row < p.rot / 16;
     // neighbouring lanes' pieces lie side by side, also where pairs are neighbours and either half would do (4 x 13020 tokens,
     // 16 / 2 heads of 160, interleaved, gradient: 273 us with each lane's pieces side by side, 186 so)
-    if (!turned) {
-      at_a = 16 * in_row, at_b = at_a + 8;
-    } else {
-      at_a = 8 * in_row, at_b = at_a + p.rot / 2;
-    }
+    if (turned) at_a = 8 * in_row, at_b = at_a + p.rot / 2;
+    else at_a = p.rot / 2 + 8 * in_row, at_b = at_a + (p.d - p.rot) / 2;
   }
   // Two sums over the lanes of a row.
   __device__ __forceinline__ void row_sums(float (&x)[2]) const {
