@@ -26,7 +26,8 @@
 // copy); its gradient 98 us (5.2 TB/s, 80 %); 32768 tokens of 64 / 8 heads to e4m3 180 us (5.0 TB/s, 78 %); rotation of
 // 16385 tokens, 16 / 16 fp16 heads of 80, 38 us (4.4 TB/s: 15 of 16 lanes hold elements, and rows start on 32 bytes); one
 // token 5.6 us.  Factors in shared memory instead of registers, for 16 to 20 warps on an SM: 72 to 108 us for the first.
-// Streaming stores and deeper rings change nothing; four CTAs on an SM spill (gradient 176 us).
+// Streaming stores and deeper rings change nothing; four CTAs on an SM spill (gradient 176 us).  A half-rotated head takes what
+// a whole one does: 4 x 8192 tokens, 16 / 4 heads of 128, 61 us, gradient 95 us.
 #include <cuda_fp16.h>
 #include <math.h>
 
