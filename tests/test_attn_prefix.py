@@ -258,6 +258,26 @@ def test_scores_far_above_the_first_tile(cuda, fp8, where):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rise", [9, 12, 40, 72, -18, -24])
+def test_scores_that_rise_within_a_segment(cuda, fp8, rise):
+    """Powers of two, so that scores are exact: some keys are 2^rise against the first tile's, within and beyond what its
+    reference leaves room for."""
+    B, Hq, S, d = 160, 12, 640, 128
+    t = make(B, Hq, 1, 1, 130, S, d, fp8)
+    for n, value in (("q", 1.0), ("k", 0.0), ("k_prefix", 0.0)):
+        x = torch.zeros(t[n].shape, device="cuda")
+        x[..., 0] = value
+        if n != "q":
+            late = slice(64, None) if rise < 0 else slice(x.shape[2] - 20, x.shape[2] - 17)
+            x[:, :, late, 0] = rise
+        t[n] = x.to(t[n].dtype)
+        if fp8:
+            t[n + "_descale"] = torch.ones_like(t[n + "_descale"])
+    check(t, wk.attn_fwd_shared_prefix(**t, softmax_scale=math.log(2)), softmax_scale=math.log(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
 def test_options_and_layouts(cuda, fp8):
     B, Hq, Hkv, Nq, P, S, d = 4, 6, 3, 2, 210, 90, 128
     t = make(B, Hq, Hkv, Nq, P, S, d, fp8)

@@ -22,8 +22,8 @@
 // Numerics: logits in base 2; statistics, sums and parts in fp32.  P is rounded to 16 bits for the tensor core: by 2^-8 of
 // itself in bf16, 2^-11 in f16; the row sums take it before that.  Tensor-core kernel: the row reference is the maximum of
 // the CTA's first tile; a CTA in which a row rises more than 2^60 above it (bf16 has the exponent range) goes through its
-// keys once more, with the maxima it then knows.  FP8: f16 P is stored times 2^5 and may rise 2^10; one below 2^-19 of the
-// reference is off by 2^-30 of it at most.  Kernel for few rows: the reference moves when a score exceeds it by more than 1;
+// keys once more, with the maxima it then knows.  FP8: f16 P is stored times 2^3 and may rise 2^12; one below 2^-17 of the
+// reference is off by 2^-28 of it at most.  Kernel for few rows: the reference moves when a score exceeds it by more than 1;
 // P is bf16, or f16 times 2^14 for FP8 inputs, whose K and V become f16 (exact).
 //
 // What bounds it.  The prefix kernel: 1090 cycles per 128 x 64 tile and SM, where the exponentials need 512 and the products
@@ -55,7 +55,7 @@ constexpr int X_S_COLS = 64;  // buffer b at column 64 b; P over its first 32
 constexpr int X_O_COL = 128;
 // How far (as a power of two) a row may rise above its reference before the CTA goes through its keys again, and what P is
 // stored times: bf16 has the exponent range, f16 (FP8 inputs) needs a larger P for the small probabilities.
-constexpr float X_MAX_EXP = 60.f, X_MAX_EXP_F16 = 10.f, X_SHIFT_F16 = 5.f, X_SHIFT_AGAIN = 14.f;
+constexpr float X_MAX_EXP = 60.f, X_MAX_EXP_F16 = 12.f, X_SHIFT_F16 = 3.f, X_SHIFT_AGAIN = 14.f;
 constexpr int X_CLUSTER = 16;  // largest cluster
 constexpr int X_PAD = 4;       // values between rows in the exchange: lanes with neighbouring rows write without conflicts
 
