@@ -17,11 +17,21 @@ _constants = {}
 
 
 def cached_tensor(key, make):
-    """A read-only constant tensor, built by ``make()`` the first time ``key`` is seen."""
+    """A read-only constant tensor, built by ``make()`` the first time ``key`` is seen.
+
+    What is kept holds its values already, so that any stream may read it.  Inside a capture, which only records how they are
+    written, a tensor is made that belongs to the capture.
+    """
     try:
         return _constants[key]
     except KeyError:
-        return _constants.setdefault(key, make())
+        made = make()
+    if made.is_cuda:
+        with torch.cuda.device(made.device):
+            if torch.cuda.is_current_stream_capturing():
+                return made
+        torch.cuda.current_stream(made.device).synchronize()
+    return _constants.setdefault(key, made)
 
 
 def check_descale(x, batch, h_kv, name):
