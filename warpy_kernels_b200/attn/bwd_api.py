@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from ..arch import require
-from ..utils import autotune, cached_tensor, check_descale
+from ..utils import autotune, cached_tensor, check_descale, packed_copy
 from .fwd_api import _check_qkv, _check_shapes, _kernel_view
 
 
@@ -34,7 +34,7 @@ def _bf16_view(x):
     """bf16 tensor the prep kernel can address: last stride 1, other strides multiples of 4 elements, 8-byte base."""
     x = x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16)
     ok = x.stride(3) == 1 and x.data_ptr() % 8 == 0 and all(st % 4 == 0 for st in x.stride()[:3])
-    return x if ok else x.contiguous()
+    return x if ok else packed_copy(x)
 
 
 def make_attn_bwd(

@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from ..arch import require
-from ..utils import any_tuned, autotune, cached_tensor, check_descale, round_up, tune_key, tune_lookup
+from ..utils import any_tuned, autotune, cached_tensor, check_descale, packed_copy, round_up, tune_key, tune_lookup
 
 BM = 128
 
@@ -48,7 +48,7 @@ def _kernel_view(x):
     because TMA zero-fills past the end of the sequence.
     """
     direct = x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(st % 16 == 0 for st in x.stride()[:3])
-    return x if direct else x.contiguous()
+    return x if direct else packed_copy(x)
 
 
 def _check_qkv(q, k, v):

@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib
 from ..arch import require
-from ..utils import cached_tensor, check_descale
+from ..utils import cached_tensor, check_descale, packed_copy
 from .fwd_api import _check_qkv, _kernel_view
 
 
@@ -31,7 +31,7 @@ class _PrefixArgs(ctypes.Structure):
 def _view(x):
     """``x`` where the kernels can read it: as ``_kernel_view``, with strides of its own along every dimension."""
     x = _kernel_view(x)
-    return x if all(st > 0 for st in x.stride()[:3]) else x.contiguous()
+    return x if all(st > 0 for st in x.stride()[:3]) else packed_copy(x)
 
 
 def attn_fwd_shared_prefix(

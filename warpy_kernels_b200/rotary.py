@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 from .arch import require
+from .utils import packed_copy
 
 _DTYPES = {torch.bfloat16: _lib.WK_BF16, torch.float16: _lib.WK_F16, torch.float32: _lib.WK_F32}
 MAX_AXES = 4
@@ -197,7 +198,7 @@ def _forward(what, q, k, q_weight, k_weight, positions, inv_freq, eps, sections,
             if x.numel() and not same and a0 < b1 and b0 < a1:
                 raise ValueError(f"{name}_out may be {name} itself but must not overlap it otherwise")
         outs.append(out)
-        src = x if _direct(x, 16) else x.contiguous()
+        src = x if _direct(x, 16) else packed_copy(x)
         dst = out if _direct(out, 8 if fp8 else 16) else torch.empty(out.shape, dtype=dtype, device=out.device)
         if dst is not out:
             copies.append((out, dst))
@@ -329,7 +330,7 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_fr
             grads.append(None)
             dws.append(None)
             continue
-        src, dsrc = (t if _direct(t, 16) else t.contiguous() for t in (x, dy))
+        src, dsrc = (t if _direct(t, 16) else packed_copy(t) for t in (x, dy))
         w = _weight(w)
         grads.append(torch.empty_like(x))
         dws.append(torch.empty_like(w))

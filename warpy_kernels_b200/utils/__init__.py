@@ -34,6 +34,15 @@ def cached_tensor(key, make):
     return _constants.setdefault(key, made)
 
 
+def packed_copy(x):
+    """A copy of ``x`` in its own order, on an allocation's boundary.
+
+    ``x.contiguous()`` is ``x`` itself where torch takes it to be contiguous, whatever its base and whatever strides its
+    dimensions of size 1 have, which the kernels' loads may not allow.
+    """
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def check_descale(x, batch, h_kv, name):
     """Accept ``None`` or a CUDA tensor shaped ``[B, Hkv]`` as a dequantisation scale.
 
