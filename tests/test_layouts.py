@@ -61,7 +61,7 @@ def test_rotation(cuda, form, B, N, dtype):
     out = torch.zeros_like(q)
     wk.rope(form(q), form(k), pos, freq, q_out=form(out))
     same(wk.qk_norm_rope(form(q), form(k), w, w, pos, freq), wk.qk_norm_rope(q, k, w, w, pos, freq))
-    same(wk.qk_norm_rope_bwd(form(dq), form(dk), q, k, w, w, pos, freq), wk.qk_norm_rope_bwd(dq, dk, q, k, w, w, pos, freq))
+    same(wk.qk_norm_rope_bwd(form(dq), form(dk), form(q), form(k), w, w, pos, freq), wk.qk_norm_rope_bwd(dq, dk, q, k, w, w, pos, freq))
     into = form(torch.zeros_like(q))
     got = wk.rope(q, k, pos, freq, q_out=into)
     assert got[0] is into
@@ -99,3 +99,19 @@ def test_attention_over_a_shared_prefix(cuda, form, B, N, fp8):
     # a dimension of size 1 without a stride
     flat = [x.as_strided(x.shape, (0, *x.stride()[1:])) for x in (kp, vp)]
     same(wk.attn_fwd_shared_prefix(q, *flat, k, v), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [1, 24])
+def test_gradients_of_rows_whose_elements_lie_apart(cuda, dtype, N):
+    """``[B, H, d, N]`` seen as ``[B, H, N, d]``: read and written, in the forward and in the backward."""
+    B, d = 2, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, dq, dk = (torch.randn(B, h, d, N, device="cuda", generator=g).to(dtype).transpose(2, 3) for h in (4, 2, 4, 2))
+    w = torch.randn(d, device="cuda", generator=g).to(dtype)
+    pos, freq = torch.arange(N, device="cuda"), torch.rand(32, device="cuda", generator=g)
+    flat = [x.clone(memory_format=torch.contiguous_format) for x in (dq, dk, q, k)]
+    same((x.contiguous() for x in wk.qk_norm_rope(q, k, w, w, pos, freq)), wk.qk_norm_rope(*flat[2:], w, w, pos, freq))
+    got, want = (wk.qk_norm_rope_bwd(*x, w, w, pos, freq) for x in ((dq, dk, q, k), flat))
+    assert all(x.shape == y.shape and torch.equal(x, y) for x, y in zip(got, want))

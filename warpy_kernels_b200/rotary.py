@@ -332,7 +332,8 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, q_weight, k_weight, positions, inv_fr
             continue
         src, dsrc = (t if _direct(t, 16) else packed_copy(t) for t in (x, dy))
         w = _weight(w)
-        grads.append(torch.empty_like(x))
+        grad = torch.empty_like(x)  # of the memory layout of x, where the kernel can write that
+        grads.append(grad if _direct(grad, 16) else torch.empty(x.shape, dtype=x.dtype, device=x.device))
         dws.append(torch.empty_like(w))
         _put(args, name, src)
         _put(args, f"d{name}_out", dsrc)
