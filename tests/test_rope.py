@@ -494,3 +494,31 @@ def turned_by_product(x, cos, sin):
     pairs = cos.shape[-1]
     a, b = x[..., :pairs], x[..., pairs : 2 * pairs]
     return torch.cat((a * cos - b * sin, b * cos + a * sin, x[..., 2 * pairs :]), -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale, eps", [(1e14, EPS), (1e17, 0.0), (1e-14, 0.0), (1e-17, 0.0), (1e-14, 1e-30)])
+def test_gradients_of_large_and_small_rows(cuda, dtype, scale, eps):
+    """Rows whose squares float32 holds, but not the third power of their norm or of its inverse."""
+    B, N, H, d, pairs = 2, 9, 3, 64, 32
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q = (scale * torch.randn(B, H, N, d, device="cuda", generator=g)).to(dtype)
+    dy = torch.randn(B, H, N, d, device="cuda", generator=g).to(dtype)
+    w = (1 + 0.3 * torch.randn(d, device="cuda", generator=g)).to(dtype)
+    pos, freq = torch.arange(N, device="cuda"), frequencies(pairs)
+    cos, sin = turn_matrix(pos.expand(B, N), freq)
+    x, w64, dy64 = q.double(), w.double(), dy.double()
+    r = (x.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    want, terms = turned(x * r * w64, cos, sin, False), pair_size(x * r * w64, pairs, False)
+    got = wk.qk_norm_rope(q, None, w, None, pos, freq, eps=eps)[0]
+    assert bool(((got.double() - want).abs() <= half_step(dtype) * want.abs() + 48 * U32 * terms).all())
+    gr, big = turned(dy64, cos, sin, False, back=True), pair_size(dy64, pairs, False)
+    h, big_h = gr * w64, big * w64.abs()
+    dx = r * (h - x * r * (h * x * r).mean(-1, keepdim=True))
+    terms = r * (big_h + (x * r).abs() * (big_h * (x * r).abs()).mean(-1, keepdim=True))
+    gx, _, gw, _ = wk.qk_norm_rope_bwd(dy, None, q, None, w, None, pos, freq, eps=eps)
+    err, bound = (gx.double() - dx).abs(), half_step(dtype) * dx.abs() + 96 * U32 * terms
+    assert bool((err <= bound).all()), (err / bound).max().item()
+    dw, dw_terms = (gr * x * r).sum((0, 1, 2)), (big * (x * r).abs()).sum((0, 1, 2))
+    assert bool(((gw.double() - dw).abs() <= half_step(dtype) * dw.abs() + 200 * U32 * dw_terms).all())

@@ -596,13 +596,14 @@ norm_rope_bwd_kernel(const __grid_constant__ RopeParams p) {
           for (int j = 0; j < 8; ++j) h[j] = mul_f32x2(g[j], w[j]);
           float sum[2] = {dot(x, x), dot(h, x)};
           at.row_sums(sum);
-          const float f = rsqrtf(sum[0] * inv_d + p.eps), m = -f * f * f * sum[1] * inv_d;
+          // dx = r (h - (x r) mean(h x r)): r^3 by itself leaves fp32 where x is beyond 1e13 or below 1e-13
+          const float f = rsqrtf(sum[0] * inv_d + p.eps), m = -f * (f * sum[1] * inv_d);
           const uint64_t f2 = pack_f32x2(f, f), m2 = pack_f32x2(m, m);
           if (there > i * p.hb) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               dw[j] = fma_f32x2(mul_f32x2(g[j], x[j]), f2, dw[j]);
-              h[j] = fma_f32x2(x[j], m2, mul_f32x2(h[j], f2));
+              h[j] = mul_f32x2(fma_f32x2(x[j], m2, h[j]), f2);
             }
             T* dst = i ? to + apart : to;
             store8(dst, h);
