@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import warpy_kernels as wk
-from warpy_kernels_b200.utils import packed_copy
+from warpy_kernels_b200.utils import overlap, packed_copy
 
 FP8 = torch.float8_e4m3fn
 
@@ -115,3 +115,28 @@ def test_gradients_of_rows_whose_elements_lie_apart(cuda, dtype, N):
     same((x.contiguous() for x in wk.qk_norm_rope(q, k, w, w, pos, freq)), wk.qk_norm_rope(*flat[2:], w, w, pos, freq))
     got, want = (wk.qk_norm_rope_bwd(*x, w, w, pos, freq) for x in ((dq, dk, q, k), flat))
     assert all(x.shape == y.shape and torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_overlap_against_all_addresses():
+    """Random shapes and strides, of one and two bytes an element, against the sets of their bytes."""
+    g = torch.Generator().manual_seed(5)
+    some = lambda values, n: [values[i] for i in torch.randint(len(values), (n,), generator=g).tolist()]
+    memory = torch.zeros(2000, dtype=torch.uint8)
+
+    def bytes_of(x):
+        at = torch.full((1,), x.data_ptr())
+        for st, n in zip(x.stride(), x.shape):
+            at = (at[:, None] + st * x.element_size() * torch.arange(n)).flatten()
+        return set((at[:, None] + torch.arange(x.element_size())).flatten().tolist())
+
+    met = 0
+    for _ in range(1500):
+        a, b = (memory.view(t).as_strided(some((1, 2, 3, 4), 4), some((0, 1, 2, 3, 4, 6, 12, 16, 24, 48), 4), some(range(60), 1)[0])
+                for t in some((torch.uint8, torch.int16), 2))
+        want = bool(bytes_of(a) & bytes_of(b))
+        met += want
+        assert overlap(a, b) == overlap(b, a) == want
+    assert 300 < met < 1200
+    x = torch.empty(3, 50, 12, 64).transpose(1, 2)  # a projection's output: its parts share none, its halves in time neither
+    assert not overlap(x[:, :4], x[:, 4:8]) and overlap(x[:, :5], x[:, 4:8]) and overlap(x, x)
+    assert not overlap(x[:, :, :25], x[:, :, 25:]) and not overlap(x[:0], x) and not overlap(x[..., :32], x[..., 32:])

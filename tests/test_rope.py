@@ -522,3 +522,37 @@ def test_gradients_of_large_and_small_rows(cuda, dtype, scale, eps):
     assert bool((err <= bound).all()), (err / bound).max().item()
     dw, dw_terms = (gr * x * r).sum((0, 1, 2)), (big * (x * r).abs()).sum((0, 1, 2))
     assert bool(((gw.double() - dw).abs() <= half_step(dtype) * dw.abs() + 200 * U32 * dw_terms).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_outputs_over_one_another(cuda, fp8):
+    """An output over the other input or the other output is refused; parts of one tensor that share no byte are not."""
+    B, N, Hq, Hkv, d = 2, 33, 4, 2, 64
+    q, k, g = inputs(B, N, Hq, Hkv, d, torch.bfloat16, "qkv")
+    pos, freq = torch.arange(N, device="cuda"), frequencies(32)
+    s = torch.full((B, Hkv), 0.02, device="cuda")
+    opts = dict(q_descale=s, k_descale=s) if fp8 else {}
+    dtype = FP8 if fp8 else torch.bfloat16
+    want = wk.rope(q, k, pos, freq, **opts)
+    store = torch.zeros(B, N, Hq + Hkv, d, device="cuda").to(dtype)
+    both = store.transpose(1, 2)
+    got = wk.rope(q, k, pos, freq, q_out=both[:, Hkv:], k_out=both[:, :Hkv], **opts)  # heads side by side
+    for x, y in zip(got, want):
+        assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))
+    before = store.view(torch.uint8).clone()
+    w = torch.ones(d, device="cuda")
+    odd = lambda x: torch.zeros(B, x.shape[1], N, d + 1, device="cuda").to(x.dtype)[..., 1:].copy_(x)  # left to the Python code
+    for a, b in ((q, k), (odd(q), odd(k))):
+        bad = [dict(q_out=both[:, :Hq], k_out=both[:, Hq - 1 : Hq - 1 + Hkv]), dict(q_out=both[:, :Hq], k_out=both[:, :Hkv])]
+        if not fp8:
+            bad += [dict(q_out=b.expand(B, Hkv, N, d).repeat(1, 2, 1, 1)[:, :Hq], k_out=a[:, 1 : 1 + Hkv])]
+            if a is q:
+                qkv = q._base.transpose(1, 2)  # [B, Hq + 2 Hkv, N, d], k behind q
+                bad += [dict(q_out=qkv[:, 1 : 1 + Hq]), dict(q_out=qkv[:, 2 * Hkv :]), dict(q_out=qkv[:, Hkv : Hkv + Hq], k_out=k)]
+        for outs in bad:
+            with pytest.raises(ValueError, match="overlap"):
+                wk.rope(a, b, pos, freq, **opts, **outs)
+            with pytest.raises(ValueError, match="overlap"):
+                wk.qk_norm_rope(a, b, w, w, pos, freq, **opts, **outs)
+    assert torch.equal(store.view(torch.uint8), before)

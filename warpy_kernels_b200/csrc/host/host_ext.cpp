@@ -600,14 +600,46 @@ bool apart(const at::Tensor& t) {
   }
 }
 
+// Whether two tensors of four dimensions share a byte; also true where that takes long to tell.  As `overlap` of
+// utils/__init__.py, where the method stands.
+struct Overlap {
+  int64_t stride[8], most[8], rest[9];  // terms of the sum: stride, number of values less one; what the later ones reach
+  int terms = 0, steps = 4096;
+  int64_t target;
+  void add(const at::Tensor& t, bool back) {
+    const int64_t size = t.element_size();
+    for (int i = 0; i < 4; ++i) {
+      const int64_t st = t.stride(i) * size, n = t.size(i) - 1;
+      if (!n || !st) continue;
+      if (back) target += st * n;
+      int at = 0;
+      while (at < terms && stride[at] > st) ++at;
+      if (at == terms || stride[at] != st) {
+        for (int j = terms++; j > at; --j) stride[j] = stride[j - 1], most[j] = most[j - 1];
+        stride[at] = st, most[at] = 0;
+      }
+      most[at] += n;
+    }
+  }
+  bool reached(int i, int64_t low, int64_t high) {
+    if (--steps < 0) return true;
+    if (i == terms) return low <= 0 && 0 <= high;
+    const int64_t need = low - rest[i + 1], first = need > 0 ? (need + stride[i] - 1) / stride[i] : 0;
+    const int64_t last = high < 0 ? -1 : std::min(most[i], high / stride[i]);
+    for (int64_t x = first; x <= last; ++x)
+      if (reached(i + 1, low - x * stride[i], high - x * stride[i])) return true;
+    return false;
+  }
+  Overlap(const at::Tensor& a, const at::Tensor& b)
+      : target(static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr())) {
+    add(a, false), add(b, true);
+    rest[terms] = 0;
+    for (int i = terms - 1; i >= 0; --i) rest[i] = rest[i + 1] + stride[i] * most[i];
+  }
+};
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  auto bytes = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int i = 0; i < t.dim(); ++i) last += t.stride(i) * (t.size(i) - 1);
-    return (last + 1) * static_cast<int64_t>(t.element_size());
-  };
-  const char *x = static_cast<const char*>(a.data_ptr()), *y = static_cast<const char*>(b.data_ptr());
-  return x < y + bytes(b) && y < x + bytes(a);
+  Overlap o(a, b);
+  return o.reached(0, o.target - static_cast<int64_t>(a.element_size()) + 1, o.target + static_cast<int64_t>(b.element_size()) - 1);
 }
 
 // The position axis of every pair, two bits each, and the number of axes (0: positions have no axis).
@@ -737,7 +769,9 @@ PyObject* rope_forward(const at::Tensor* q, const at::Tensor* k, PyObject* q_out
           !rope_rows(*t, fp8 ? 8 : 16) || !apart(*t))
         return declined();
       const bool same = t->data_ptr() == x->data_ptr() && t->strides() == x->strides() && dtype == x->scalar_type();
-      if (!same && overlap(*t, *x)) return declined();
+      const at::Tensor* other = i ? q : k;
+      if ((!same && overlap(*t, *x)) || (other && overlap(*t, *other)) || (i && outs[0].defined() && overlap(*t, outs[0])))
+        return declined();
       outs[i] = *t;
     }
   }

@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .arch import require
-from .utils import packed_copy
+from .utils import apart, overlap, packed_copy
 
 _DTYPES = {torch.bfloat16: _lib.WK_BF16, torch.float16: _lib.WK_F16, torch.float32: _lib.WK_F32}
 MAX_AXES = 4
@@ -38,21 +38,6 @@ def _direct(x, unit):
     """Whether the kernels can address ``x``: last stride 1, base and other strides multiples of ``unit`` bytes."""
     size = x.element_size()
     return x.stride(3) == 1 and x.data_ptr() % unit == 0 and all(st * size % unit == 0 for st in x.stride()[:3])
-
-
-def _apart(x):
-    """Whether no two elements of ``x`` share memory: every stride spans what the smaller ones reach."""
-    span = 1
-    for st, n in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
-        if st < span:
-            return False
-        span = st * n
-    return True
-
-
-def _range(x):
-    first = x.data_ptr()
-    return first, first + (sum(st * (n - 1) for st, n in zip(x.stride(), x.shape)) + 1) * x.element_size()
 
 
 def _check_heads(name, x, like, dtype):
@@ -191,12 +176,14 @@ def _forward(what, q, k, q_weight, k_weight, positions, inv_freq, eps, sections,
         if out is None:
             out = torch.empty_like(x, dtype=dtype)
         else:
-            if out.shape != x.shape or out.dtype != dtype or out.device != x.device or not _apart(out):
+            if out.shape != x.shape or out.dtype != dtype or out.device != x.device or not apart(out):
                 raise ValueError(f"{name}_out must be a {dtype} tensor shaped like {name} whose elements do not share memory")
             same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and out.dtype == x.dtype
-            (a0, a1), (b0, b1) = _range(x), _range(out)
-            if x.numel() and not same and a0 < b1 and b0 < a1:
+            if not same and overlap(out, x):
                 raise ValueError(f"{name}_out may be {name} itself but must not overlap it otherwise")
+            for other, y in (("k", k), ("k_out", k_out)) if name == "q" else (("q", q),):
+                if y is not None and y.device == out.device and overlap(out, y):
+                    raise ValueError(f"{name}_out must not overlap {other}")
         outs.append(out)
         src = x if _direct(x, 16) else packed_copy(x)
         dst = out if _direct(out, 8 if fp8 else 16) else torch.empty(out.shape, dtype=dtype, device=out.device)
@@ -244,7 +231,8 @@ def rope(q, k, positions, inv_freq, sections=None, cycle=False, interleaved=Fals
         interleaved: Pair ``j`` is elements ``2 j`` and ``2 j + 1``. ``False``: elements ``j`` and ``j + pairs``.
         inverse: Turn back. That is the gradient: ``rope(dq, dk, ..., inverse=True)``.
         q_out: Output like ``q``, any strides, such as ``q`` itself. ``None`` allocates one with the memory layout of ``q``.
-        k_out: The same for ``k``, such as a part of a cache. Outputs must not overlap anything but their own input.
+        k_out: The same for ``k``, such as a part of a cache. Outputs must not share a byte with anything but their own input;
+            parts of one tensor that lie between one another are fine.
         q_descale: ``[B, Hkv]`` float32: write e4m3 codes of ``q / q_descale``, saturated at 448, which ``attn_fwd`` takes
             with the same descale. ``None``: outputs have the dtype of ``q``.
         k_descale: The same for ``k``. Give both or none.
@@ -253,7 +241,8 @@ def rope(q, k, positions, inv_freq, sections=None, cycle=False, interleaved=Fals
         ``(q, k)``, turned; the second is ``None`` if ``k`` is.
 
     Raises:
-        ValueError: If a dtype, shape, device or section does not fit, or an output overlaps its input.
+        ValueError: If a dtype, shape, device or section does not fit, or an output shares a byte with an input or the other
+            output without being its own input.
         NotImplementedError: If the GPU is not supported.
     """
     done = _lib.host().rope(q, k, positions, inv_freq, sections, cycle, interleaved, inverse, q_out, k_out, q_descale, k_descale)
@@ -279,7 +268,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, sectio
         ``(q, k)``, the second ``None`` if ``k`` is.
 
     Raises:
-        ValueError: If a dtype, shape, device or section does not fit, or an output overlaps its input.
+        ValueError: If a dtype, shape, device or section does not fit, or an output shares a byte with an input or the other
+            output without being its own input.
         NotImplementedError: If the GPU is not supported.
     """
     done = _lib.host().qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps, sections, cycle, interleaved, q_out,

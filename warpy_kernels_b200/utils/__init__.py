@@ -43,6 +43,51 @@ def packed_copy(x):
     return x.clone(memory_format=torch.contiguous_format)
 
 
+def apart(x):
+    """Whether no two elements of ``x`` share memory: every stride spans what the smaller ones reach."""
+    span = 1
+    for st, n in sorted((st, n) for st, n in zip(x.stride(), x.shape) if n > 1):
+        if st < span:
+            return False
+        span = st * n
+    return True
+
+
+def overlap(a, b):
+    """Whether two tensors share a byte, by their addresses, shapes and strides; also true where that takes long to tell.
+
+    An element of ``a`` and one of ``b`` meet if the sum of ``stride * index`` over the dimensions of both, those of ``b``
+    counted negative, is within an element's size of the distance of their bases.  Dimensions of equal stride make one term,
+    and for each value of the term with the largest stride the others must reach what is left: one or two values each for
+    tensors whose strides span what the smaller ones reach, such as parts of one projection's output.
+    """
+    if not a.numel() or not b.numel():
+        return False
+    size_a, size_b = a.element_size(), b.element_size()
+    target, terms = b.data_ptr() - a.data_ptr(), {}  # stride: the sum's number of values less one
+    for x, size, sign in ((a, size_a, 1), (b, size_b, -1)):
+        for st, n in zip(x.stride(), x.shape):
+            if n > 1 and st:
+                terms[st * size] = terms.get(st * size, 0) + n - 1
+                target += st * size * (n - 1) if sign < 0 else 0  # indices of b counted from their ends
+    terms = sorted(terms.items(), reverse=True)
+    steps = 4096
+
+    def reached(i, low, high):
+        nonlocal steps
+        steps -= 1
+        if steps < 0:
+            return True
+        if i == len(terms):
+            return low <= 0 <= high
+        stride, most = terms[i]
+        rest = sum(st * n for st, n in terms[i + 1 :])
+        first, last = max(0, -((rest - low) // stride)), min(most, high // stride)
+        return any(reached(i + 1, low - x * stride, high - x * stride) for x in range(first, last + 1))
+
+    return reached(0, target - size_a + 1, target + size_b - 1)
+
+
 def check_descale(x, batch, h_kv, name):
     """Accept ``None`` or a CUDA tensor shaped ``[B, Hkv]`` as a dequantisation scale.
 
