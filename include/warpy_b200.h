@@ -378,7 +378,8 @@ int wk_qk_norm_rope_bwd(const wk_rope_args* args, void* stream);
  *   seqused_k [B] int32 or NULL: how many of its S own keys each sequence attends to
  *   q_descale, k_descale, v_descale [B,Hkv], k_prefix_descale, v_prefix_descale [Hkv]  fp32 contiguous, fp8 only
  *   causal: query i of a sequence with n own keys sees the first P + n - Nq + i + 1 keys of [prefix ; own]
- *   out [B,Hq,Nq,d] bf16, 8-byte aligned, element strides multiples of 4; lse fp32 or NULL, element strides (B, H)
+ *   out [B,Hq,Nq,d] bf16, 8-byte aligned, element strides multiples of 4, which may be q (bf16, the same strides) but must
+ *       not overlap anything else; lse fp32 or NULL, element strides (B, H)
  *   workspace: wk_attn_fwd_shared_prefix_workspace_bytes, 16-byte aligned; holds nothing between calls; calls that can run
  *       at the same time need buffers of their own
  * Rows without a visible key get out = 0, lse = +inf.  Keys and values must be finite where a row sees them; what lies

@@ -465,3 +465,43 @@ def test_refusals(cuda):
             wk.attn_fwd_shared_prefix(q8, kp8, kp8, k8, k8, **change)
     with pytest.raises(TypeError):
         wk.attn_fwd_shared_prefix(q, kp, kp, k, k, no_such_option=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq", [1, 9, 40])
+def test_the_output_in_place_of_the_queries(cuda, Nq):
+    """``out`` may be ``q``; anything else that it shares a byte with is refused, and so is one that overlaps itself."""
+    B, Hq, Hkv, P, S, d = 3, 8, 2, 700, 300, 128
+    t = make(B, Hq, Hkv, Nq, P, S, d, False, layout="bnhd")
+    want = wk.attn_fwd_shared_prefix(**t)
+    room = torch.zeros(B, Nq + 1, Hq + 2, d + 16, device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    inside = dict(t) | dict(q=room[:, 1:-1, :Nq, :d].copy_(t["q"]))
+    for call in (inside, dict(t)):
+        got = wk.attn_fwd_shared_prefix(**call, out=call["q"])
+        assert got[0] is call["q"] and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = room[:, 1:-1, :Nq, :d].copy_(want[0])
+    t["q"] = q
+    store = torch.zeros(B * Hq * (Nq + 1) * d + 64, device="cuda", dtype=torch.bfloat16)
+    memory = dict(q=q, k=t["k"], v=t["v"], k_prefix=t["k_prefix"], v_prefix=t["v_prefix"])
+    for name, x in memory.items():
+        base = x._base if x._base is not None else x
+        flat = base.as_strided((base.untyped_storage().nbytes() // 2,), (1,), 0)
+        if flat.numel() < B * Hq * Nq * d + 16:
+            continue
+        for out in (flat[8 : 8 + B * Hq * Nq * d].view(B, Hq, Nq, d), flat[4 : 4 + B * Hq * Nq * d].view(B, Nq, Hq, d).transpose(1, 2)):
+            with pytest.raises(ValueError, match="overlap " + name):
+                wk.attn_fwd_shared_prefix(**t, out=out)
+    for out in (store.as_strided((B, Hq, Nq, d), (64, 4, d * Hq, 1)), store[:d].expand(B, Hq, Nq, d)):
+        with pytest.raises(ValueError, match="share memory"):
+            wk.attn_fwd_shared_prefix(**t, out=out)
+    between = room[:, 1:-1, 1:, :d]  # tokens one behind the queries': over them, unless there is but one
+    if Nq == 1:
+        assert torch.equal(wk.attn_fwd_shared_prefix(**t, out=between)[0], wk.attn_fwd_shared_prefix(**t)[0])
+    else:
+        with pytest.raises(ValueError, match="overlap q"):
+            wk.attn_fwd_shared_prefix(**t, out=between)
+    t8 = make(B, Hq, Hkv, Nq, P, S, d, True)
+    wide = torch.zeros(B, Hq, Nq, 2 * d, device="cuda", dtype=torch.uint8)
+    t8["q"] = wide.view(FP8)[..., :d].copy_(t8["q"])
+    with pytest.raises(ValueError, match="overlap q"):
+        wk.attn_fwd_shared_prefix(**t8, out=wide.view(torch.bfloat16))

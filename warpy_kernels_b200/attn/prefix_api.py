@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib
 from ..arch import require
-from ..utils import cached_tensor, check_descale, packed_copy
+from ..utils import apart, cached_tensor, check_descale, overlap, packed_copy
 from .fwd_api import _check_qkv, _kernel_view
 
 
@@ -58,8 +58,8 @@ def attn_fwd_shared_prefix(
         causal: Whether query ``i`` sees only the first ``P + n - Nq + i + 1`` keys of the prefix and the ``n`` own keys of
             its sequence (the bottom-right aligned mask of ``attn_fwd``).
         softmax_scale: Scale on the logits, positive. Defaults to ``1 / sqrt(d)``.
-        out: Output buffer, ``[B, Hq, Nq, d]`` bf16 with last stride 1. ``None`` allocates one with the memory layout of
-            ``q``.
+        out: Output buffer, ``[B, Hq, Nq, d]`` bf16 with last stride 1, such as ``q`` itself; it must not share a byte with
+            anything else. ``None`` allocates one with the memory layout of ``q``.
         return_lse: Whether to compute ``lse``.
         seqused_k: ``[B]`` int32, how many of its ``S`` own keys each sequence attends to; ``None`` for all. It is read on
             the device (a captured graph sees later values). What ``k`` and ``v`` hold behind them is never used.
@@ -70,7 +70,7 @@ def attn_fwd_shared_prefix(
         or ``None`` without ``return_lse``. Rows with no visible key get 0 and ``+inf``.
 
     Raises:
-        ValueError: If a dtype, shape, device or option does not fit.
+        ValueError: If a dtype, shape, device or option does not fit, or ``out`` overlaps an input without being ``q``.
         NotImplementedError: If the GPU does not support the dtype of ``q``.
     """
     done = _lib.host().attn_fwd_shared_prefix(q, k_prefix, v_prefix, k, v, q_descale, k_descale, v_descale, k_prefix_descale,
@@ -114,8 +114,13 @@ def attn_fwd_shared_prefix(
         raise ValueError("seqused_k must be an int32 CUDA tensor of shape [B]")
     if out is None:
         out = torch.empty_like(q, dtype=torch.bfloat16)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(3) != 1:
-        raise ValueError("out must be a bf16 tensor shaped like q with last stride 1")
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(3) != 1 or not apart(out):
+        raise ValueError("out must be a bf16 tensor shaped like q, with last stride 1, whose elements do not share memory")
+    else:
+        for name, x in zip(names, tensors):
+            same = x is tensors[0] and out.data_ptr() == x.data_ptr() and out.stride() == x.stride() and not fp8
+            if not same and overlap(out, x):
+                raise ValueError(f"out must not overlap {name}" + (" without being it" if name == "q" else ""))
     args = _PrefixArgs()
     views = [_view(x) for x in tensors]
     direct = out.data_ptr() % 8 == 0 and all(st > 0 and st % 4 == 0 for st in out.stride()[:3])

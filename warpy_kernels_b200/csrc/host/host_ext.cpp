@@ -916,6 +916,11 @@ PyObject* attn_fwd_shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t na
       return declined();
     for (int i = 0; i < 3; ++i)
       if (o->stride(i) < 1 || o->stride(i) % 4) return declined();
+    if (!apart(*o)) return declined();
+    for (const at::Tensor* x : {q, kp, vp, k, v}) {
+      const bool same = x == q && o->data_ptr() == q->data_ptr() && o->strides() == q->strides() && !s.fp8;
+      if (!same && overlap(*o, *x)) return declined();
+    }
     out = *o;
   } else {
     out = like(*q, at::kBFloat16);
