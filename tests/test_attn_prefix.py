@@ -505,3 +505,22 @@ def test_the_output_in_place_of_the_queries(cuda, Nq):
     t8["q"] = wide.view(FP8)[..., :d].copy_(t8["q"])
     with pytest.raises(ValueError, match="overlap q"):
         wk.attn_fwd_shared_prefix(**t8, out=wide.view(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Nq", [1, 12])
+def test_repeats_itself_beside_other_work(cuda, fp8, Nq):
+    """Rings that are refilled while they are read: the same bits every time, also while another stream keeps the memory busy."""
+    t = make(7, 8, 8, Nq, 300, 3000, 128, fp8)
+    want = wk.attn_fwd_shared_prefix(**t)
+    check(t, want)
+    side, copy = torch.cuda.Stream(), torch.empty(2, 1 << 28, device="cuda", dtype=torch.uint8)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            copy[0].copy_(copy[1])
+    got = [wk.attn_fwd_shared_prefix(**t) for _ in range(40)]
+    torch.cuda.synchronize()
+    for out, lse in got:
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])

@@ -1098,9 +1098,12 @@ attn_prefix_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
           }
         }
       }
-      // Into V's place, which every lane has read once it has a sum that its last fragment went into.  The vote waits for
-      // that; which lane then issues the load is all the same.
-      fetch(C::SLOTS % 2 == 0, __any_sync(0xffffffffu, o[NT - 1][C::K16 - 1][0] == -1.23456789e-30f) ? 1 : 0);
+      // Into V's place, once every lane has read all of it: the vote is over bits of a sum of each fragment of V.  Which lane
+      // then issues the load is all the same.
+      uint32_t seen = 0;
+#pragma unroll
+      for (int k = 0; k < C::K16; k += FP8 ? 2 : 1) seen |= __float_as_uint(o[NT - 1][k][0]);  // FP8: one fragment for two
+      fetch(C::SLOTS % 2 == 0, __any_sync(0xffffffffu, seen == 0xffffffffu) ? 1 : 0);
     }
 
     // ---- this warp's part: O / l and the log-sum-exp
