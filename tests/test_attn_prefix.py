@@ -524,3 +524,31 @@ def test_repeats_itself_beside_other_work(cuda, fp8, Nq):
     torch.cuda.synchronize()
     for out, lse in got:
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8, Nq, P, S", [
+    (True, 1, 600, 0), (True, 1, 0, 600), (True, 12, 0, 600), (True, 40, 0, 600), (True, 1, 6000, 90), (False, 1, 600, 0),
+    (False, 1, 0, 600), (False, 40, 0, 600)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_bits_of_the_probabilities(cuda, fp8, Nq, P, S, d):
+    """Two thirds of the keys have one and the same probability against the others', (1 + 2^-8 + 2^-12) / 2, and values of the
+    other sign, so that the sums nearly cancel and what its rounding leaves is all there is to see: 2^-11 of sum p |v| at most
+    in f16 (FP8 inputs), 2^-8 in bf16, which here would be off by 2^-9.  Beside that the exponential (2^-21), one float32
+    addition (2^-23) for every 16 keys, and the output's rounding."""
+    B, Hq, Hkv = 3, 2, 1
+    dtype = FP8 if fp8 else torch.bfloat16
+    x = (1 + 2.0**-8 + 2.0**-12) / 2
+    q = torch.zeros(B, Hq, Nq, d, device="cuda")
+    q[..., 0] = 1
+    t = dict(q=q)
+    for b, n, names in ((1, P, ("k_prefix", "v_prefix")), (B, S, ("k", "v"))):
+        small = (torch.arange(n, device="cuda") % 3 != 0)[None, None, :, None].expand(b, Hkv, n, d).float()
+        t[names[0]], t[names[1]] = -small * (torch.arange(d, device="cuda") == 0), 1 - 2 * small
+    t = {n: y.to(dtype) for n, y in t.items()}
+    out, _ = wk.attn_fwd_shared_prefix(**t, softmax_scale=-math.log(x))
+    T = P + S
+    many = sum(int((torch.arange(n) % 3 != 0).sum()) for n in (P, S))
+    want = ((T - many) - many * x) / ((T - many) + many * x)
+    err = (out.double() - want).abs().max().item()
+    assert err <= 2.0**-8 * abs(want) + (2.0**-11 if fp8 else 2.0**-8) + 2.0**-21 + T / 16 * 2.0**-23  # sum p |v| is 1

@@ -15,9 +15,9 @@
 // prefix kernel is set up and runs beside the one for own keys and waits for its end before it reads its parts.
 //
 // One CTA of the tensor-core kernel (two per SM, 320 threads): warp 0 TMA producer, warp 1 issues the products, two softmax
-// groups of four warps take the tiles in turn, one thread per row: the structure of attn_fwd_bf16.cu.  P is bf16 and
-// overwrites its scores in tensor memory.  FP8: scores from e4m3 (kind::f8f6f4); V tiles become f16 (exact) in shared memory,
-// by the group that has the tile and while its scores are computed, and P is f16.
+// groups of four warps take the tiles in turn, one thread per row: the structure of attn_fwd_bf16.cu.  P has 16 bits and
+// overwrites its scores in tensor memory.  BF16: P is bf16.  FP8: scores from e4m3 (kind::f8f6f4); V tiles become f16 (exact)
+// in shared memory, by the group that has the tile and while its scores are computed, and P is f16.
 //
 // Numerics: logits in base 2; statistics, sums and parts in fp32.  P is rounded to 16 bits for the tensor core: by 2^-8 of
 // itself in bf16, 2^-11 in f16; the row sums take it before that.  Tensor-core kernel: the row reference is the maximum of
@@ -159,14 +159,14 @@ template <bool FP8, int DH>
 struct PrefixCfg {
   static constexpr int SIZE = FP8 ? 1 : 2;
   static constexpr int SPANS = FP8 ? 1 : DH / 64;      // 128-byte spans of a K row
-  static constexpr int V_SPANS = DH / 64;              // of a V row in bf16
+  static constexpr int V_SPANS = DH / 64;              // of a V row in 16 bits
   static constexpr int Q_SPAN = X_ROWS * 128;          // bytes
   static constexpr int KV_SPAN = X_KEYS * 128;
   static constexpr int Q_BYTES = SPANS * Q_SPAN;
   static constexpr int K_BYTES = SPANS * KV_SPAN;      // of a stage; V as loaded likewise
   static constexpr int V16_BYTES = V_SPANS * KV_SPAN;
   static constexpr int STAGES = FP8 || DH == 128 ? 2 : 4;
-  static constexpr int V16S = 3;  // FP8: buffers of V in bf16
+  static constexpr int V16S = 3;  // FP8: buffers of V in f16
   static constexpr int Q_AT = 0;
   static constexpr int K_AT = Q_BYTES;
   static constexpr int V_AT = K_AT + STAGES * K_BYTES;
@@ -407,7 +407,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
         const int tile = J + j;
         const int st = tile % ST, key0 = (tile0 + j) * X_KEYS;
         if (FP8) {
-          // This tile of V to bf16, while its scores are computed: a thread takes half a row, neighbours' stores in different
+          // This tile of V to f16, while its scores are computed: a thread takes half a row, neighbours' stores in different
           // banks.  Rows behind the last key become zeros, whatever the cache holds there: 0 . V has to be 0.
           const int buf = tile % C::V16S;
           ok = ok && mbar_wait_warp(v_full(st), (tile / ST) & 1, p.status, WK_ERR_TIMEOUT_LOAD) &&
