@@ -78,14 +78,6 @@ template <>
 struct Raw<float> {
   float4 a0, a1, b0, b1;
 };
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 // A warp's 512 elements in the ring: 16-byte pieces, lane after lane.
 template <typename T>
 constexpr int kRowBytes = 512 * sizeof(T);
