@@ -125,3 +125,33 @@ def test_what_is_made_inside_a_capture_is_not_kept(monkeypatch):
     assert utils.cached_tensor("key", make) is kept
     host = utils.cached_tensor("other", lambda: torch.ones(2))  # on the host there is nothing to wait for
     assert utils.cached_tensor("other", lambda: None) is host
+
+
+@pytest.mark.gpu
+def test_graphs_that_run_beside_one_another_share_no_flags(cuda):
+    """The forward marks query blocks to be computed again in a buffer that one call at a time may use."""
+    from warpy_kernels_b200 import _lib
+
+    host, graphs, seen = _lib.host(), [torch.cuda.CUDAGraph() for _ in range(2)], []
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v = (torch.randn(2, 8, 700, 64, device="cuda", generator=g).bfloat16() for _ in range(3))
+    k[:, :, 650] *= 60  # rows that rise beyond their reference's range
+    want = wk.attn_fwd(q, k, v)
+    outs = []
+    for graph in graphs:  # on one stream, one after the other
+        with torch.cuda.graph(graph):
+            outs.append([wk.attn_fwd(q, k, v) for _ in range(2)])
+            seen.append({host.block_flags(0, 64).data_ptr(), host.block_flags(0, 64).data_ptr()})
+    seen.append({host.block_flags(0, 64).data_ptr()})
+    assert all(len(x) == 1 for x in seen) and len(set.union(*seen)) == 3
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(10):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    assert all(torch.equal(x, y) for x, y in zip(wk.attn_fwd(q, k, v), want))
+    torch.cuda.synchronize()
+    for calls in outs:
+        for got in calls:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -170,10 +170,22 @@ int on_device(int dev, F fn) {
 // ---- attention --------------------------------------------------------------------------------------------------
 // Zeroed scratch for the forward's block flags, one per (device, stream): the kernels hand it back zeroed, so the
 // calls that follow one another on a stream share it.  Torch has a fixed number of streams per device, which bounds
-// the table; a buffer only ever grows.  Guarded by the GIL.
+// the table; a buffer only ever grows.  Graphs may be replayed beside one another and beside other calls, whatever stream
+// they were captured on: a capture has a buffer of its own, in its graph's memory, whose zeros are part of the graph.  The
+// table keeps it as long as calls of that capture may come.  Guarded by the GIL.
 at::Tensor& block_flags(int dev, void* stream, int64_t nbytes) {
-  static auto* table = new std::map<std::pair<int, void*>, at::Tensor>();  // outlives the interpreter's teardown
-  at::Tensor& buf = (*table)[{dev, stream}];
+  struct Buffers {
+    at::Tensor eager, captured;
+    unsigned long long capture = 0;
+  };
+  static auto* table = new std::map<std::pair<int, void*>, Buffers>();  // outlives the interpreter's teardown
+  Buffers& b = (*table)[{dev, stream}];
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  const bool capturing = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture) == cudaSuccess &&
+                         status == cudaStreamCaptureStatusActive;
+  if (capturing && b.capture != capture) b.captured = at::Tensor(), b.capture = capture;
+  at::Tensor& buf = capturing ? b.captured : b.eager;
   if (!buf.defined() || buf.numel() < nbytes)
     buf = at::zeros({std::max<int64_t>(nbytes, 1 << 16)},
                     at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(dev)));
