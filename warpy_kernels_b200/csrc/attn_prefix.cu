@@ -28,9 +28,13 @@
 //
 // What bounds it.  The prefix kernel: 1090 cycles per 128 x 64 tile and SM, where the exponentials need 512 and the products
 // 400 to 640 (ncu: MUFU 50 %, tensor pipe 37 %, issue slots 52 %): the chain scores -> P -> product with two groups in each
-// of two CTAs.  128 rows of 8 heads over 32768 keys 130 us FP8, 135 us bf16 (530 / 510 TFLOP/s).  (V to bf16 by integer
-// arithmetic instead, behind the scores: 164 us; 128-key tiles in one CTA per SM, tensor memory read ahead, waits that poll: no
-// faster.)  Own keys: their bytes in bf16 (97 us for 537 MB), the latency of a warp's instructions in FP8 (64 us for 268 MB).
+// of two CTAs (at 96 registers a thread, 12 to 152 bytes of them read back from local memory).  128 sequences, 64 / 8 heads,
+// so 1024 stacked rows of each of 8 heads, over 32768 keys: 135 us FP8, 141 us bf16 a call (1020 / 975 TFLOP/s).  (V to bf16
+// by integer arithmetic instead, behind the scores: 164 where the present form then took 130; 128-key tiles in one CTA per
+// SM, tensor memory read ahead, waits that poll: no faster.)
+// Those are for logits of 1.5 nats' spread.  In FP8 a rise of 2^12 is 8.3 nats: with a wider spread more CTAs go through their
+// keys twice.  The same call at 1.5, 2, 2.5, 3 and 4 nats: 139, 189, 227, 256, 257 us FP8, 144 to 145 bf16 (2^60).
+// Own keys: their bytes in bf16 (97 us for 537 MB), the latency of a warp's instructions in FP8 (64 us for 268 MB).
 // Whole calls, inputs from HBM: 16 sequences, 64 / 8 heads, 8192 shared and up to 1024 own bf16 keys 26.5 us; 128 sequences,
 // 32768 and up to 2048 FP8 keys 200 to 210 us; 24 sequences, 32 / 8 heads, 5 queries, 4096 and up to 512 bf16 keys 38 us;
 // 64 sequences, 32 heads, 2048 and up to 300 FP8 keys 33.5 us.

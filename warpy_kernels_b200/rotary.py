@@ -222,8 +222,9 @@ def rope(q, k, positions, inv_freq, sections=None, cycle=False, interleaved=Fals
         k: ``[B, Hkv, N, d]`` of the same dtype, or ``None``.
         positions: ``[B, N]`` int32 or int64, or ``[N]`` for all batch items. With ``sections`` one such tensor per axis:
             ``[axes, B, N]`` or ``[axes, N]``.
-        inv_freq: ``[pairs]`` float32 or float64: angle per position of each pair, with whatever scaling a model gives it.
-            ``pairs`` is a multiple of 8; the first ``2 * pairs`` elements of a head are turned, the others left.
+        inv_freq: ``[pairs]`` float32 or float64: angle per position of each pair, with whatever scaling a model gives its
+            angles (one that multiplies cosine and sine goes into the norm's weights or ``softmax_scale``, where a whole head
+            is turned). ``pairs`` is a multiple of 8; the first ``2 * pairs`` elements of a head are turned, the others left.
         sections: How many pairs each position axis turns (time, height, width), up to four, adding up to ``pairs``.
             ``None``: one axis.
         cycle: Pairs take the axes in turn (pair ``j`` axis ``j % axes``) for as long as an axis has pairs left, then the
