@@ -552,3 +552,14 @@ def test_bits_of_the_probabilities(cuda, fp8, Nq, P, S, d):
     want = ((T - many) - many * x) / ((T - many) + many * x)
     err = (out.double() - want).abs().max().item()
     assert err <= 2.0**-8 * abs(want) + (2.0**-11 if fp8 else 2.0**-8) + 2.0**-21 + T / 16 * 2.0**-23  # sum p |v| is 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("B, Hq, Hkv, Nq, P, S, d", [(3, 4, 2, 512, 700, 512, 128), (2, 2, 1, 777, 130, 900, 64), (1, 3, 3, 300, 0, 300, 128)])
+def test_prompts_behind_a_prefix(cuda, fp8, B, Hq, Hkv, Nq, P, S, d):
+    """Hundreds of queries a sequence, most of whose tiles the causal mask cuts."""
+    t = make(B, Hq, Hkv, Nq, P, S, d, fp8, layout="bnhd")
+    check(t, wk.attn_fwd_shared_prefix(**t, causal=True), True)
+    used = torch.tensor([S, Nq // 2, 1][:B], device="cuda", dtype=torch.int32)  # and sequences shorter than their queries
+    check(t, wk.attn_fwd_shared_prefix(**t, causal=True, seqused_k=used), True, used)

@@ -182,8 +182,11 @@ at::Tensor& block_flags(int dev, void* stream, int64_t nbytes) {
   Buffers& b = (*table)[{dev, stream}];
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   unsigned long long capture = 0;
-  const bool capturing = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture) == cudaSuccess &&
-                         status == cudaStreamCaptureStatusActive;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &capture) != cudaSuccess) {
+    cudaGetLastError();  // whatever it is, the launch will tell
+    status = cudaStreamCaptureStatusNone;
+  }
+  const bool capturing = status == cudaStreamCaptureStatusActive;
   if (capturing && b.capture != capture) b.captured = at::Tensor(), b.capture = capture;
   at::Tensor& buf = capturing ? b.captured : b.eager;
   if (!buf.defined() || buf.numel() < nbytes)

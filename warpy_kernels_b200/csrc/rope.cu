@@ -510,7 +510,7 @@ rope_kernel(const __grid_constant__ RopeParams p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           turn(v[i], own, other, at.turned, p.interleaved, y);
-          if (FP8) f[i] *= __frcp_rn(scale[i]);
+          if (FP8) f[i] *= __frcp_rn(scale[i]);  // within 2^-23 of the quotient, which moves codes that close to a tie
           if (NORM || FP8) {
             const uint64_t f2 = pack_f32x2(f[i], f[i]);
 #pragma unroll
